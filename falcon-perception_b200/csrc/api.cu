@@ -61,6 +61,8 @@ int make_epilogue(const fpkv_epilogue* e, int n_q_heads, Epilogue* out) {
     return FPKV_OK;
 }
 
+inline bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
 int check_arch() {
     int dev = 0, major = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return FPKV_EARCH;
@@ -292,6 +294,94 @@ int fpkv_prefill_attn(const fpkv_pool* pool, int32_t layer, void* out, float* ls
                                  sm_scale, epi, status, static_cast<cudaStream_t>(stream));
     return launch_prefill_portable(pv, layer, out, lse, q, q_stride_h, q_stride_t, batch_idx, extent, L, n_q_heads,
                                    sm_scale, epi, status, static_cast<cudaStream_t>(stream));
+}
+
+// What fpkv_decode_attn_shared and its workspace query refuse in the same way.
+static int check_shared(const PoolView& pv, int32_t B, int32_t n_q_heads, int32_t n_groups)
+{
+    if (B < 0 || n_q_heads <= 0 || n_groups < 0) return FPKV_EINVAL;
+    if (pv.dtype != FPKV_BF16 && pv.dtype != FPKV_F16) return FPKV_EDTYPE;
+    if (n_q_heads % pv.H || n_groups > FPKV_MAX_GROUPS || !decode_shared_supported(pv, n_q_heads)) return FPKV_ESHAPE;
+    // grids are B * n_q_heads blocks wide and positions are 32-bit on the device
+    if ((long long)B * n_q_heads > (1ll << 24) || (long long)pv.n_pages * pv.P >= (1ll << 31)) return FPKV_ESHAPE;
+    return FPKV_OK;
+}
+
+int fpkv_decode_shared_workspace_bytes(const fpkv_pool* pool, int32_t B, int32_t n_q_heads, int32_t n_groups, size_t* bytes)
+{
+    PoolView pv;
+    int rc = make_view(pool, 0, &pv);
+    if (rc) return rc;
+    if (bytes == nullptr) return FPKV_EINVAL;
+    if ((rc = check_shared(pv, B, n_q_heads, n_groups))) return rc;
+    *bytes = decode_shared_workspace_bytes(pv, B, n_q_heads, n_groups) + 256;
+    return FPKV_OK;
+}
+
+int fpkv_decode_attn_shared(const fpkv_pool* pool, int32_t layer, void* out, float* lse, const void* q,
+                            int64_t q_stride_b, int64_t q_stride_h, const int64_t* batch_idx, const void* input_pos,
+                            int32_t pos_type, int32_t B, int32_t n_q_heads, const int32_t* groups, int32_t n_groups,
+                            const int32_t* row_group, float sm_scale, void* workspace, size_t workspace_bytes,
+                            const fpkv_epilogue* epilogue, int32_t* status, void* stream)
+{
+    PoolView pv;
+    int rc = make_view(pool, layer, &pv);
+    if (rc) return rc;
+    Epilogue epi;
+    if ((rc = make_epilogue(epilogue, n_q_heads, &epi))) return rc;
+    if (pos_type != FPKV_I32 && pos_type != FPKV_I64) return FPKV_EINVAL;
+    if ((rc = check_shared(pv, B, n_q_heads, n_groups))) return rc;
+    if (B == 0) return FPKV_OK;
+    if (out == nullptr || lse == nullptr || batch_idx == nullptr || input_pos == nullptr || workspace == nullptr)
+        return FPKV_EINVAL;
+    if (n_groups > 0 && (groups == nullptr || row_group == nullptr)) return FPKV_EINVAL;
+    if ((rc = check_rows(q, q_stride_b, q_stride_h, pv.esize))) return rc;
+    if (!aligned16(out) || !aligned16(workspace) || !aligned16(groups) || !aligned_to(row_group, 4)) return FPKV_EALIGN;
+    if (workspace_bytes < decode_shared_workspace_bytes(pv, B, n_q_heads, n_groups)) return FPKV_EWORKSPACE;
+    if ((rc = check_arch())) return rc;
+    return launch_decode_shared(pv, layer, out, lse, q, q_stride_b, q_stride_h, batch_idx, input_pos, pos_type, B,
+                                n_q_heads, groups, n_groups, row_group, sm_scale, workspace, epi, status,
+                                static_cast<cudaStream_t>(stream));
+}
+
+int fpkv_step_tables(const fpkv_pool* pool, const int64_t* slots, const int32_t* starts, const int32_t* lens,
+                     int32_t n_req, int32_t row_tokens, int32_t align, int32_t width, const int64_t* tokens,
+                     int64_t n_tokens, int64_t pad_id, const fpkv_step_out* out, int32_t* status, void* stream)
+{
+    PoolView pv;
+    int rc = make_view(pool, 0, &pv);
+    if (rc) return rc;
+    if (out == nullptr || n_req < 0 || row_tokens < 0 || align <= 0 || width < 0 || n_tokens < 0) return FPKV_EINVAL;
+    if (n_req > FPKV_MAX_REQUESTS || row_tokens > (1 << 30) || align > (1 << 20)) return FPKV_ESHAPE;
+    if (n_req > 0 && (slots == nullptr || starts == nullptr || lens == nullptr)) return FPKV_EINVAL;
+    if (tokens == nullptr && n_tokens > 0) return FPKV_EINVAL;
+    if (!aligned_to(slots, 8) || !aligned_to(starts, 4) || !aligned_to(lens, 4) || !aligned_to(tokens, 8) ||
+        !aligned_to(out->input_ids, 8) || !aligned_to(out->input_pos, 8) || !aligned_to(out->batch_idx, 8) ||
+        !aligned_to(out->pool_row, 8) || !aligned_to(out->block_table, 4) || !aligned_to(out->seq_lens, 4) ||
+        !aligned_to(out->offsets, 4) || !aligned_to(out->last, 4))
+        return FPKV_EALIGN;
+    if ((rc = check_arch())) return rc;
+    return launch_step_tables(pv, slots, starts, lens, n_req, row_tokens, align, width, tokens, n_tokens, pad_id, *out,
+                              status, static_cast<cudaStream_t>(stream));
+}
+
+int fpkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const float* uniform,
+                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* token,
+                float* logprob, void* stream)
+{
+    const int es = esize_of(dtype);
+    if (es == 0) return FPKV_EDTYPE;
+    if (rows < 0 || vocab <= 0) return FPKV_EINVAL;
+    if (vocab > (1 << 24) || (rows > 1 && row_stride < vocab)) return FPKV_ESHAPE;
+    if (rows == 0) return FPKV_OK;
+    if (logits == nullptr || uniform == nullptr || token == nullptr) return FPKV_EINVAL;
+    if (!aligned_to(logits, es) || !aligned_to(uniform, 4) || !aligned_to(temperature, 4) || !aligned_to(top_k, 4) ||
+        !aligned_to(top_p, 4) || !aligned_to(min_p, 4) || !aligned_to(token, 8) || !aligned_to(logprob, 4))
+        return FPKV_EALIGN;
+    const int rc = check_arch();
+    if (rc) return rc;
+    return launch_sample(logits, dtype, row_stride, rows, vocab, uniform, temperature, top_k, top_p, min_p, token, logprob,
+                         static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

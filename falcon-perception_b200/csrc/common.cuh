@@ -135,4 +135,18 @@ int launch_prefill_tc(const PoolView& pv, int layer, void* out, float* lse, cons
                       long long q_stride_t, const int64_t* batch_idx, const int32_t* extent, int L, int Hq,
                       float sm_scale, const Epilogue& epi, int32_t* status, cudaStream_t stream);
 
+
+bool decode_shared_supported(const PoolView& pv, int Hq);
+size_t decode_shared_workspace_bytes(const PoolView& pv, int B, int Hq, int n_groups);
+int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, const void* q, long long q_stride_b,
+                         long long q_stride_h, const int64_t* batch_idx, const void* pos, int pos_type, int B, int Hq,
+                         const int32_t* groups, int n_groups, const int32_t* row_group, float sm_scale, void* workspace,
+                         const Epilogue& epi, int32_t* status, cudaStream_t stream);
+int launch_step_tables(const PoolView& pv, const int64_t* slots, const int32_t* starts, const int32_t* lens, int n_req,
+                       int row_tokens, int align, int width, const int64_t* tokens, int64_t n_tokens, int64_t pad_id,
+                       const fpkv_step_out& out, int32_t* status, cudaStream_t stream);
+int launch_sample(const void* logits, int dtype, long long row_stride, int rows, int vocab, const float* uniform,
+                  const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* token,
+                  float* logprob, cudaStream_t stream);
+
 }  // namespace fpkv

@@ -26,7 +26,7 @@ constexpr int kAllocThreads = 512;
 constexpr int kAllocWarps = kAllocThreads / 32;
 constexpr int kMaxOpsPerLaunch = 2048;
 
-enum : int { kOpAllocate = 0, kOpReserve = 1, kOpErase = 2, kOpMap = 3, kOpClear = 4 };
+enum : int { kOpAllocate = 0, kOpReserve = 1, kOpErase = 2, kOpMap = 3, kOpClear = 4, kOpShare = 5, kOpRelease = 6 };
 
 __global__ void __launch_bounds__(kAllocThreads)
 alloc_step_kernel(int64_t* __restrict__ page_table, int64_t* __restrict__ p2l, int n_pages, int max_batch,
@@ -56,6 +56,14 @@ alloc_step_kernel(int64_t* __restrict__ page_table, int64_t* __restrict__ p2l, i
             } else if (op.x == kOpErase) {                 // a = pages the slot owns (logical 0 .. a-1)
                 if (op.z < 0 || op.z > n_pages || np + op.z > n_pages || ns >= max_batch) raise_status(status, FPKV_STATUS_BAD_PAGE);
                 else { base = np; np += op.z; free_slots[ns++] = op.y; }
+            } else if (op.x == kOpRelease) {               // a = pages the slot holds, the first b of them shared and kept
+                const int back = op.z - op.w;
+                if (op.z < 0 || op.z > n_pages || op.w < 0 || back < 0 || np + back > n_pages || ns >= max_batch) raise_status(status, FPKV_STATUS_BAD_PAGE);
+                else { base = np; np += back; free_slots[ns++] = op.y; }
+            } else if (op.x == kOpShare) {                 // a = slot whose pages are shared, b = how many
+                if (op.z <= 0 || op.z >= max_batch || op.z == op.y) raise_status(status, FPKV_STATUS_BAD_SLOT);
+                else if (op.w < 0 || op.w > n_pages) raise_status(status, FPKV_STATUS_BAD_PAGE);
+                else base = 0;
             } else if (op.x == kOpMap) {                   // a = logical page, b = physical page (page 0 is reserved)
                 if (op.z < 0 || op.z >= n_pages || op.w <= 0 || op.w >= n_pages) raise_status(status, FPKV_STATUS_BAD_PAGE);
                 else base = 0;
@@ -78,9 +86,21 @@ alloc_step_kernel(int64_t* __restrict__ page_table, int64_t* __restrict__ p2l, i
         if (k == n_ops) break;
         const int kind = s_op[k].x;
         int i1 = k + 1;
-        if (kind == kOpReserve || kind == kOpErase)
+        if (kind == kOpReserve || kind == kOpErase || kind == kOpRelease)
             while (i1 < n_ops && (s_op[i1].x == kind || s_op[i1].x == kOpAllocate)) ++i1;
-        if (kind == kOpClear) {                                // both rows in full, all threads
+        if (kind == kOpShare) {                                // one record at a time: its source may be an earlier record's target
+            if (s_base[k] >= 0) {
+                const int4 op = s_op[k];
+                const int64_t* src = page_table + (size_t)op.z * n_pages;
+                int64_t* pt = page_table + (size_t)op.y * n_pages;
+                int64_t* il = p2l + (size_t)op.y * n_pages;
+                for (int j = tid; j < op.w; j += kAllocThreads) {
+                    const long long pg = src[j];
+                    if (pg <= 0 || pg >= n_pages) { raise_status(status, FPKV_STATUS_BAD_PAGE); continue; }
+                    pt[j] = pg; il[pg] = j;
+                }
+            }
+        } else if (kind == kOpClear) {                         // both rows in full, all threads
             if (s_base[k] >= 0) {
                 int64_t* pt = page_table + (size_t)s_op[k].y * n_pages;
                 int64_t* il = p2l + (size_t)s_op[k].y * n_pages;
@@ -103,6 +123,13 @@ alloc_step_kernel(int64_t* __restrict__ page_table, int64_t* __restrict__ p2l, i
                     for (int j = lane; j < op.z; j += 32) {
                         const long long pg = pt[j];
                         free_pages[base + (op.z - 1 - j)] = (int)pg;
+                        pt[j] = -1;
+                        if (pg > 0 && pg < n_pages) il[pg] = -1; else raise_status(status, FPKV_STATUS_BAD_PAGE);
+                    }
+                } else if (op.x == kOpRelease) {               // as an erase, but the first b pages stay with their other holders
+                    for (int j = lane; j < op.z; j += 32) {
+                        const long long pg = pt[j];
+                        if (j >= op.w) free_pages[base + (op.z - 1 - j)] = (int)pg;
                         pt[j] = -1;
                         if (pg > 0 && pg < n_pages) il[pg] = -1; else raise_status(status, FPKV_STATUS_BAD_PAGE);
                     }

@@ -26,8 +26,10 @@ STATUS_BAD_SLOT, STATUS_BAD_POS, STATUS_BAD_PAGE, STATUS_TIMEOUT, STATUS_OPEN_SP
 # every symbol include/fpkv.h declares
 EXPORTS = ("fpkv_version", "fpkv_build_id", "fpkv_strerror", "fpkv_alloc_step", "fpkv_append_decode", "fpkv_append_packed",
            "fpkv_pre_append", "fpkv_gather", "fpkv_decode_workspace_bytes", "fpkv_decode_attn", "fpkv_decode_attn_static",
-           "fpkv_prefill_attn")
-OP_ALLOCATE, OP_RESERVE, OP_ERASE, OP_MAP, OP_CLEAR = 0, 1, 2, 3, 4
+           "fpkv_prefill_attn", "fpkv_decode_shared_workspace_bytes", "fpkv_decode_attn_shared", "fpkv_step_tables",
+           "fpkv_sample")
+OP_ALLOCATE, OP_RESERVE, OP_ERASE, OP_MAP, OP_CLEAR, OP_SHARE, OP_RELEASE = 0, 1, 2, 3, 4, 5, 6
+MAX_GROUPS, MAX_REQUESTS = 1024, 4096
 
 
 class FpkvPool(ctypes.Structure):
@@ -47,6 +49,12 @@ class FpkvAllocState(ctypes.Structure):
 class FpkvEpilogue(ctypes.Structure):
     """struct fpkv_epilogue"""
     _fields_ = [("sinks", ctypes.c_void_p), ("sinks_dtype", ctypes.c_int32), ("token_major", ctypes.c_int32)]
+
+
+class FpkvStepOut(ctypes.Structure):
+    """struct fpkv_step_out"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("input_ids", "input_pos", "batch_idx", "pool_row", "block_table", "seq_lens",
+                                               "offsets", "last")]
 
 
 class FpkvError(RuntimeError):
@@ -99,6 +107,15 @@ def _load():
     lib.fpkv_prefill_attn.argtypes = [pool, i32, vp, vp, vp, i64, i64, vp, vp, i32, i32, f32, i32, epi, vp, vp]
     lib.fpkv_decode_attn_static.restype = ctypes.c_int
     lib.fpkv_decode_attn_static.argtypes = [pool, i32, vp, vp, vp, i64, i64, vp, vp, i32, i32, i32, f32, vp, vp]
+    lib.fpkv_decode_shared_workspace_bytes.restype = ctypes.c_int
+    lib.fpkv_decode_shared_workspace_bytes.argtypes = [pool, i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)]
+    lib.fpkv_decode_attn_shared.restype = ctypes.c_int
+    lib.fpkv_decode_attn_shared.argtypes = [pool, i32, vp, vp, vp, i64, i64, vp, vp, i32, i32, i32, vp, i32, vp, f32, vp,
+                                            ctypes.c_size_t, epi, vp, vp]
+    lib.fpkv_step_tables.restype = ctypes.c_int
+    lib.fpkv_step_tables.argtypes = [pool, vp, vp, vp, i32, i32, i32, i32, vp, i64, i64, ctypes.POINTER(FpkvStepOut), vp, vp]
+    lib.fpkv_sample.restype = ctypes.c_int
+    lib.fpkv_sample.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
     return lib
 
 

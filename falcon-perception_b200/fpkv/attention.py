@@ -33,18 +33,33 @@ class CausalDecodeMask:
     def seq_lengths(self):
         return (self.L, self.L)
 
-    def for_step(self, batch_idx: Tensor, input_pos: Tensor) -> "DecodeStepMask":
+    def for_step(self, batch_idx: Tensor, input_pos: Tensor, shared: "PrefixGroups | None" = None) -> "DecodeStepMask":
         """The slice the reference engine takes each decode step
         (``paged_inference.py:783-826``)."""
-        return DecodeStepMask(batch_idx, input_pos, self.page_size)
+        return DecodeStepMask(batch_idx, input_pos, self.page_size, shared)
+
+
+@dataclass
+class PrefixGroups:
+    """Which rows of a decode batch share leading pages
+    (``PagedKVCache.prefix_groups``): a plan for the kernels, good as long as the
+    rows of the batch stay the same."""
+    groups: Tensor      # (G, 4) int32: first row, rows, shared pages, 0
+    row_group: Tensor   # (B,) int32: group of every row, -1 for none
+
+    @property
+    def n_groups(self):
+        return int(self.groups.shape[0])
 
 
 @dataclass
 class DecodeStepMask:
-    """Decode-step mask: slot and position of every row of the batch."""
+    """Decode-step mask: slot and position of every row of the batch, and the
+    prefixes its rows share (None: none, or not to be made use of)."""
     batch_idx: Tensor
     input_pos: Tensor
     page_size: int
+    shared: PrefixGroups | None = None
 
 
 @dataclass

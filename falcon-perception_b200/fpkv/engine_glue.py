@@ -37,18 +37,21 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
-from .attention import CausalDecodeMask, DecodeStepMask, PrefillMask
+from .attention import CausalDecodeMask, DecodeStepMask, PrefillMask, PrefixGroups
 from .paged_attention import PagedKVCache
+from .sampling import sample
 
 
 # ------------------------------------------------------------ attention call
-def decoding_block_mask(block_mask: CausalDecodeMask, batch_idx: Tensor, input_pos: Tensor) -> DecodeStepMask:
+def decoding_block_mask(block_mask: CausalDecodeMask, batch_idx: Tensor, input_pos: Tensor,
+                        shared: PrefixGroups | None = None) -> DecodeStepMask:
     """Replacement body of ``PagedInferenceEngine.get_decoding_block_mask``
     (``paged_inference.py:783-826``): the step's mask is the slot and position
-    of every row; the kernels walk the page table themselves."""
+    of every row; the kernels walk the page table themselves.  ``shared``: the
+    prefixes the rows share (``PagedKVCache.prefix_groups``)."""
     assert batch_idx.ndim == 1, "batch_idx must be 1D"
     assert input_pos.ndim == 1, "input_pos must be 1D"
-    return block_mask.for_step(batch_idx, input_pos)
+    return block_mask.for_step(batch_idx, input_pos, shared)
 
 
 def fpkv_attention_forward(self, x, attention_masks, kv_cache, freqs_cis, freqs_cis_2d=None, input_pos=None,
@@ -68,11 +71,13 @@ def fpkv_attention_forward(self, x, attention_masks, kv_cache, freqs_cis, freqs_
     B, S, _ = x.shape
     n_q, n_kv, D = self.n_kv_heads * self.n_rep, self.n_kv_heads, self.head_dim
     decode = S == 1
+    shared = attention_masks.shared if isinstance(attention_masks, DecodeStepMask) else None
     if fused:
         qkv = self.wqkv(F.rms_norm(x, (x.size(-1),)))
         xq = kv_cache.pre_attention_append(self.layer_id, qkv, n_q, n_kv, freqs_cis, freqs_cis_2d, batch_idx, input_pos)
         if decode:
-            out, _ = kv_cache.decode_attention(self.layer_id, xq, batch_idx, input_pos.reshape(-1), sinks=self.sinks)
+            out, _ = kv_cache.decode_attention(self.layer_id, xq, batch_idx, input_pos.reshape(-1), sinks=self.sinks,
+                                               shared=shared)
         else:
             out, _ = kv_cache.prefill_attention(self.layer_id, xq, batch_idx, input_pos, attention_masks,
                                                 sinks=self.sinks, token_major=True)
@@ -81,7 +86,7 @@ def fpkv_attention_forward(self, x, attention_masks, kv_cache, freqs_cis, freqs_
     if kv_cache.n_heads == n_kv and self.n_rep > 1 and not kv_cache.split_q_heads:   # each KV head stored once: drop the copies
         xk, xv = xk[:, ::self.n_rep], xv[:, ::self.n_rep]
     if decode:
-        out, lse = kv_cache.decode_step(self.layer_id, xq, xk, xv, batch_idx, input_pos)
+        out, lse = kv_cache.decode_step(self.layer_id, xq, xk, xv, batch_idx, input_pos, shared=shared)
     else:
         kv_cache.insert_kv(self.layer_id, xk, xv, input_pos=input_pos, batch_idx=batch_idx)
         out, lse = kv_cache.prefill_attention(self.layer_id, xq, batch_idx, input_pos, attention_masks)
@@ -255,6 +260,14 @@ class SlotState:
         batch_idx (bucket,), input_pos (bucket,) int32, rope_pos_t (bucket,) int64, input_ids (bucket,)."""
         bi = self.batch_idx[:bucket]
         return bi, self.input_pos[bi], self.rope_pos_t[bi], self.last_token[bi]
+
+    def sample(self, bucket: int, logits: Tensor, uniform: Tensor, temperature=None, top_k=None, top_p=None, min_p=None):
+        """Draw every row's next token (``fpkv.sampling.sample``) and move the
+        batch on (``advance``).  Device work only, in the order a captured decode
+        step has it.  Returns (token, logprob) of the bucket's rows."""
+        token, logprob = sample(logits, uniform, temperature, top_k, top_p, min_p)
+        self.advance(bucket, token)
+        return token, logprob
 
     def advance(self, bucket: int, next_token: Tensor):
         """After sampling: every live row of the batch moves on by one token.  Device work only, no

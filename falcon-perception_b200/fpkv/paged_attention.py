@@ -24,12 +24,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+from dataclasses import dataclass
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import CausalDecodeMask, DecodeStepMask, PrefillMask, image_span_ids
+from .attention import CausalDecodeMask, DecodeStepMask, PrefillMask, PrefixGroups, image_span_ids
 from .kv_cache import KVCacheBase
 
 _DTYPES = {torch.float32: _lib.FPKV_F32, torch.bfloat16: _lib.FPKV_BF16, torch.float16: _lib.FPKV_F16}
@@ -60,6 +61,19 @@ def _epilogue(sinks: Tensor | None, token_major: bool = False):
 
 def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+@dataclass
+class StepTables:
+    """Indices of one step's packed row and its requests (``PagedKVCache.step_tables``)."""
+    input_ids: Tensor | None    # (1, row_tokens) int64, None when no tokens were given
+    input_pos: Tensor           # (1, row_tokens) int64
+    batch_idx: Tensor           # (1, row_tokens) int64: slot of each token, 0 for pads
+    pool_row: Tensor            # (row_tokens,) int64: the token's row in every plane of the pool, -1 for pads
+    block_table: Tensor         # (N, width) int32: physical pages, -1 beyond the request's last
+    seq_lens: Tensor            # (N,) int32: starts + lens
+    offsets: Tensor             # (N + 1,) int32: packed index of each request's first token; the end
+    last: Tensor                # (N,) int32: packed index of each request's last token, -1 without tokens
 
 
 class PagedKVCache(KVCacheBase):
@@ -102,6 +116,7 @@ class PagedKVCache(KVCacheBase):
         self.capacity = [0 for _ in range(max_batch_size)]
         self._free_pages = list(reversed(range(1, n_pages)))
         self._free_batch_idx = list(reversed(range(1, max_batch_size)))
+        self._page_holders = {}                     # physical page -> number of slots that hold it, where more than one does
         # [slot, physical page] -> logical page
         self._physical_to_logical = torch.full((max_batch_size, n_pages), -1, dtype=torch.int64, device=device)
 
@@ -332,13 +347,55 @@ class PagedKVCache(KVCacheBase):
         self.capacity[batch_idx_int] += n_new * self.page_size
         return True
 
+    def share_prefix(self, batch_idx_int: int, n_tokens: int) -> int:
+        """Allocate a slot whose first ``n_tokens`` tokens are those of slot
+        ``batch_idx_int``, in the same pages: another request about the same
+        picture or document costs no pages and no prefill for it.  ``n_tokens`` is
+        a multiple of ``page_size`` (a page that is still being filled belongs to
+        one request) and the pages hold what the other slot appended or will
+        append; nobody may append at positions below ``n_tokens`` once they are
+        in use.  ``reserve`` then grows the new slot with pages of its own.  A
+        shared page goes back to the free list with its last holder."""
+        assert 0 < batch_idx_int < self.max_batch_size, "slot out of range"
+        assert n_tokens >= 0 and n_tokens % self.page_size == 0, "only whole pages can be shared"
+        assert n_tokens <= self.capacity[batch_idx_int], "the slot holds fewer tokens than are to be shared"
+        assert batch_idx_int not in self._free_batch_idx, "the slot is not allocated"
+        slot = self.allocate()
+        n = n_tokens // self.page_size
+        if n == 0:
+            return slot
+        pages = self.page_table_cpu[batch_idx_int][:n]
+        for pg in pages:
+            self._page_holders[pg] = self._page_holders.get(pg, 1) + 1
+        if self._dev.type == "cuda":
+            self._pending.append((_lib.OP_SHARE, slot, batch_idx_int, n))
+        else:
+            for i, pg in enumerate(pages):
+                self._page_table[slot, i] = pg
+                self._physical_to_logical[slot, pg] = i
+        self.page_table_cpu[slot] = list(pages)
+        self.capacity[slot] = n_tokens
+        return slot
+
     def erase(self, batch_idx: int) -> None:
         self._free_batch_idx.append(batch_idx)
         owned = self.page_table_cpu[batch_idx]
-        self._free_pages.extend(reversed(owned))
+        # Pages that other slots hold too stay.  They are leading ones: a slot can only share what comes first in
+        # another, so whoever holds a slot's page j holds its pages 0 .. j - 1 as well.
+        kept = 0
+        while kept < len(owned) and owned[kept] in self._page_holders:
+            pg = owned[kept]
+            self._page_holders[pg] -= 1
+            if self._page_holders[pg] == 1:
+                del self._page_holders[pg]
+            kept += 1
+        self._free_pages.extend(reversed(owned[kept:]))
         # cleared on the device too, so padding rows and stale slots read "unmapped"
         if self._dev.type == "cuda":
-            self._pending.append((_lib.OP_ERASE, batch_idx, len(owned), 0))
+            if kept:
+                self._pending.append((_lib.OP_RELEASE, batch_idx, len(owned), kept))
+            else:
+                self._pending.append((_lib.OP_ERASE, batch_idx, len(owned), 0))
         else:
             self._page_table[batch_idx, :] = -1
             self._physical_to_logical[batch_idx, :] = -1
@@ -484,7 +541,7 @@ class PagedKVCache(KVCacheBase):
 
     def decode_step(self, layer_id: int, q: Tensor, k: Tensor, v: Tensor, batch_idx: Tensor, input_pos: Tensor,
                     sm_scale: float | None = None, out: Tensor | None = None, lse: Tensor | None = None,
-                    sinks: Tensor | None = None):
+                    sinks: Tensor | None = None, shared: PrefixGroups | None = None):
         """Append k, v (B,H,1,D) and attend with q (B,Hq,1,D) in one go: what
         ``Attention.forward`` does per layer in a decode step (``insert_kv``
         followed by the attention call, ``falcon_perception/model.py:150-162``).
@@ -493,18 +550,23 @@ class PagedKVCache(KVCacheBase):
         the append instead of waiting for it.  With ``sinks`` (n_q_heads,) the
         returned out is already ``out * sigmoid(lse - sinks)``, the gate of
         ``_post_attention`` (``model.py:122-128``); viewed as (B, 1, Hq*D) it is
-        what the output projection takes."""
+        what the output projection takes.  ``shared`` as for ``decode_attention``."""
         B = q.shape[0]
         self.assign(layer_id, batch_idx, input_pos.reshape(B, 1), k, v)
-        return self.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks=sinks,
+        return self.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks=sinks, shared=shared,
                                      _after_append=True)
 
     def decode_attention(self, layer_id: int, q: Tensor, batch_idx: Tensor, input_pos: Tensor,
                          sm_scale: float | None = None, out: Tensor | None = None, lse: Tensor | None = None,
-                         sinks: Tensor | None = None, _after_append: bool = False):
+                         sinks: Tensor | None = None, shared: PrefixGroups | None = None, _after_append: bool = False):
         """One query token per row against keys 0..input_pos[b] of slot
         batch_idx[b].  q (B,Hq,1,D) -> out (B,Hq,1,D) in q's dtype, lse (B,Hq,1)
-        fp32.  Call after ``insert_kv`` of the same step, as the model does."""
+        fp32.  Call after ``insert_kv`` of the same step, as the model does.
+        ``shared`` (``prefix_groups`` of the batch's slots): leading pages that
+        rows have in common are read once for all of them; the result is the same.
+        Pools that ``fpkv_decode_attn_shared`` does not take (fp32, split layout,
+        page sizes other than 128, more than 16 query heads per stored head) are
+        served row by row as without it."""
         B, Hq, S, D = q.shape
         assert S == 1, "decode attention takes one query token per row"
         assert D == self.head_dim and Hq % self.n_heads == 0, "head layout must match the pool"
@@ -526,6 +588,11 @@ class PagedKVCache(KVCacheBase):
             out = torch.empty((B, Hq, 1, D), dtype=q.dtype, device=q.device)
         if lse is None:
             lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=q.device)
+        if shared is not None:
+            assert shared.row_group.shape == (B,), "the prefix groups are those of another batch"
+            if shared.n_groups and self._shared_supported(Hq):
+                self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared)
+                return out, lse
         ws = self._get_workspace(B, Hq)
         scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
         flags = int(self.decode_kernel) | (_lib.DECODE_AFTER_APPEND if _after_append else 0)
@@ -537,6 +604,110 @@ class PagedKVCache(KVCacheBase):
             _stream(self._dev)),
             "fpkv_decode_attn")
         return out, lse
+
+    # ----------------------------------------------------------- shared prefixes
+    def prefix_groups(self, slots, rows: int | None = None, into: PrefixGroups | None = None) -> PrefixGroups:
+        """Which consecutive rows of a decode batch have leading pages in common.
+        ``slots``: the slot of every row (host integers, in batch order; rows of
+        one prefix next to each other); ``rows``: the padded batch size, rows
+        beyond ``slots`` are in no group.  Host work and one small copy: make it
+        when the batch changes, pass it to every layer of every step until then.
+        ``into`` refills an earlier record in place (same number of rows, no more
+        groups than it has room for), so that a captured graph sees the new batch."""
+        slots = [int(s) for s in slots]
+        rows = len(slots) if rows is None else int(rows)
+        assert rows >= len(slots), "the padded batch is smaller than the batch"
+        found, row_group, i = [], [-1] * rows, 0
+        while i < len(slots):
+            first = self.page_table_cpu[slots[i]]
+            n, j = len(first), i + 1
+            while j < len(slots):
+                other = self.page_table_cpu[slots[j]]
+                m = min(n, len(other))
+                if first[:m] != other[:m]:
+                    m = next(k for k in range(m) if first[k] != other[k])
+                # one more row saves m pages a row, but cuts what the others share down to m: stop where that loses more
+                if m == 0 or (j - i > 1 and (j - i) * m < (j - i - 1) * n):
+                    break
+                n, j = m, j + 1
+            if j - i > 1:
+                row_group[i:j] = [len(found)] * (j - i)
+                found.append((i, j - i, n, 0))
+            i = j
+        if into is not None:
+            assert into.row_group.shape[0] == rows and len(found) <= into.n_groups, "the record has no room for this batch"
+            found += [(0, 0, 0, 0)] * (into.n_groups - len(found))
+        assert len(found) <= _lib.MAX_GROUPS, f"more than {_lib.MAX_GROUPS} groups"
+        flat = torch.tensor([x for g in found for x in g] + row_group, dtype=torch.int32)
+        if into is not None:
+            n = 4 * into.n_groups
+            into.groups.copy_(flat[:n].view(-1, 4))
+            into.row_group.copy_(flat[n:])
+            return into
+        flat = flat.to(self._dev)
+        return PrefixGroups(flat[:4 * len(found)].view(-1, 4), flat[4 * len(found):])
+
+    def _shared_supported(self, Hq: int) -> bool:
+        return (self.dtype != torch.float32 and not self.split_q_heads and self.page_size == 128
+                and Hq // self.n_heads <= 16)
+
+    def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared):
+        B, Hq, _, D = q.shape
+        assert shared.groups.is_cuda and shared.groups.is_contiguous() and shared.groups.dtype == torch.int32
+        assert shared.row_group.is_cuda and shared.row_group.is_contiguous() and shared.row_group.dtype == torch.int32
+        need = ctypes.c_size_t(0)
+        _lib.check(_lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(self._pool), B, Hq, shared.n_groups,
+                                                               ctypes.byref(need)), "fpkv_decode_shared_workspace_bytes")
+        # scratch of this call alone: from torch's allocator, so that calls on other streams and captured graphs have their own
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
+        epi = _epilogue(sinks)
+        _lib.check(_lib.lib.fpkv_decode_attn_shared(
+            ctypes.byref(self._pool), layer_id, out.data_ptr(), lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
+            batch_idx.data_ptr(), input_pos.data_ptr(), _pos_type(input_pos), B, Hq, shared.groups.data_ptr(),
+            shared.n_groups, shared.row_group.data_ptr(), scale, ws.data_ptr(), ws.numel(),
+            ctypes.byref(epi) if epi is not None else None, self._status_ptr(), _stream(self._dev)),
+            "fpkv_decode_attn_shared")
+
+    # ------------------------------------------------------------- step indices
+    def step_tables(self, slots: Tensor, starts: Tensor, lens: Tensor, row_tokens: int, width: int | None = None,
+                    align: int = 128, tokens: Tensor | None = None, pad_id: int = 0) -> StepTables:
+        """Packed-row indices, block tables and slot maps of a step whose request
+        lengths live on the device: request r brings tokens
+        [starts[r], starts[r] + lens[r]) of slot slots[r] (all (N,), int64 /
+        int32 / int32).  The row is laid out as ``pack_prefill_rows`` lays out
+        chunks -- every request on a multiple of ``align``, pads carry slot 0
+        and position 0 -- in ``row_tokens`` tokens, which the caller fixes (so that
+        the call can be captured); tokens that do not fit are dropped and reported
+        through ``check_status``.  ``tokens`` (int64): the requests' token ids
+        back to back.  ``width``: columns of the block table (default: n_pages).
+        The result feeds ``insert_kv``, ``pre_attention_append`` and
+        ``prefill_attention``."""
+        assert slots.ndim == 1 and starts.shape == slots.shape and lens.shape == slots.shape, "one slot, start and length a request"
+        assert slots.dtype == torch.int64, "slots must be int64"
+        assert starts.dtype == torch.int32 and lens.dtype == torch.int32, "starts and lens must be int32"
+        assert tokens is None or (tokens.dtype == torch.int64 and tokens.ndim == 1), "tokens must be one int64 row"
+        N, L = slots.shape[0], int(row_tokens)
+        W = self.n_pages if width is None else int(width)
+        assert L >= 0 and W >= 0 and align > 0, "row_tokens, width and align must not be negative"
+        assert N <= _lib.MAX_REQUESTS, f"more than {_lib.MAX_REQUESTS} requests"
+        self._require_cuda(slots, starts, lens)
+        if tokens is not None:
+            assert tokens.is_cuda, "tensor must be on the cache's CUDA device"
+            tokens = tokens.contiguous()
+        slots, starts, lens = slots.contiguous(), starts.contiguous(), lens.contiguous()
+        dev = slots.device
+        wide = torch.empty((4 if tokens is not None else 3, 1, L), dtype=torch.int64, device=dev)
+        row, pos, bidx, *ids = wide.unbind(0)
+        narrow = torch.empty(N * (W + 3) + 1, dtype=torch.int32, device=dev)
+        block, seq, last, off = narrow.split_with_sizes((N * W, N, N, N + 1))
+        out = _lib.FpkvStepOut(ids[0].data_ptr() if ids else None, pos.data_ptr(), bidx.data_ptr(), row.data_ptr(),
+                               block.data_ptr(), seq.data_ptr(), off.data_ptr(), last.data_ptr())
+        _lib.check(_lib.lib.fpkv_step_tables(
+            ctypes.byref(self._pool), slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), N, L, int(align), W,
+            tokens.data_ptr() if tokens is not None else None, tokens.numel() if tokens is not None else 0, int(pad_id),
+            ctypes.byref(out), self._status_ptr(), _stream(self._dev)), "fpkv_step_tables")
+        return StepTables(ids[0] if ids else None, pos, bidx, row[0], block.view(N, W), seq, off, last)
 
     def prefill_attention(self, layer_id: int, q: Tensor, batch_idx: Tensor, input_pos: Tensor, mask: PrefillMask,
                           sm_scale: float | None = None, sinks: Tensor | None = None, token_major: bool = False):
@@ -620,7 +791,7 @@ class PagedKVCache(KVCacheBase):
                 "batch_idx must have the same shape as block_mask"
             assert batch_idx.shape[0] <= self.max_batch_size, \
                 "batch_idx must be less than or equal to max_batch_size"
-            return DecodeStepMask(batch_idx, block_mask.input_pos, self.page_size)
+            return DecodeStepMask(batch_idx, block_mask.input_pos, self.page_size, block_mask.shared)
         return block_mask
 
     def get_logical_kv_idx(self, physical_batch_idx: Tensor, physical_kv_idx: Tensor, batch_idx: Tensor):
@@ -657,14 +828,15 @@ def paged_attention(q: Tensor, kv_cache: PagedKVCache, layer_id: int, batch_idx:
     shaped and typed like q and lse (B,Hq,S) fp32.
 
     Decode: q (B,Hq,1,D), batch_idx (B,), input_pos (B,) or (B,1); ``mask`` may
-    be the step's DecodeStepMask (its tensors are used when given).
+    be the step's DecodeStepMask (its tensors and prefix groups are used when given).
     Prefill: q (1,Hq,L,D), batch_idx and input_pos (1,L), ``mask`` the
     PrefillMask of the packed row; keys are read from the pages, so call it
     after ``insert_kv``.
     """
     if batch_idx.ndim == 1:
+        shared = None
         if isinstance(mask, DecodeStepMask):
-            batch_idx, input_pos = mask.batch_idx, mask.input_pos
-        return kv_cache.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale)
+            batch_idx, input_pos, shared = mask.batch_idx, mask.input_pos, mask.shared
+        return kv_cache.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale, shared=shared)
     assert isinstance(mask, PrefillMask), "prefill needs the mask from create_prefill_blockmask"
     return kv_cache.prefill_attention(layer_id, q, batch_idx, input_pos, mask, sm_scale)

@@ -176,6 +176,11 @@ typedef struct fpkv_alloc_state {
  *   kind 3  map       page_table[slot, a] = b; physical_to_logical[slot, b] = a
  *                     (for callers that keep their own free lists)
  *   kind 4  clear     both table rows of `slot` to -1 in full
+ *   kind 5  share     logical pages 0 .. b-1 of slot a also become logical pages
+ *                     0 .. b-1 of `slot` (which holds none); nothing is popped
+ *   kind 6  release   erase of a slot whose first b pages other slots still hold:
+ *                     as kind 2 with a pages, but only the pages of logical
+ *                     pages b .. a-1 go back to the stack
  * Slot 0 and page 0 are reserved and never edited; records naming them, ids
  * out of range, a pop that does not give `slot`, or a reserve beyond the
  * stack are skipped and raise FPKV_STATUS_BAD_SLOT / _BAD_PAGE.
@@ -387,6 +392,113 @@ FPKV_API int fpkv_decode_attn_static(const fpkv_pool* pool, int32_t layer,
                                      const int64_t* batch_idx, const void* input_pos, int32_t pos_type,
                                      int32_t B, int32_t n_q_heads, float sm_scale,
                                      int32_t* status, void* stream);
+
+/*
+ * Paged decode attention for a batch whose rows share long prefixes: several
+ * requests about one picture or document, their first pages mapped to the same
+ * physical pages (allocator record "share").  It has no counterpart in the
+ * reference.  Same results and conventions as fpkv_decode_attn on the same
+ * arguments; the keys of a shared prefix are read once for all rows of its
+ * group instead of once a row.
+ *   groups     device int32 [n_groups][4], 16-byte aligned, each {first row, rows,
+ *              shared pages, 0}: batch rows first .. first+rows-1 all map logical
+ *              pages 0 .. shared-1 to the same physical pages (the kernel reads
+ *              them through the first row's slot).  Groups do not overlap; one
+ *              with no rows or no shared pages is skipped.
+ *   row_group  device int32 [B]: the group of every row, -1 for none.  A row whose
+ *              entry does not name a group that contains it counts as in none.
+ * Both are device data: a captured call may be replayed with other contents.
+ * A row's position may lie anywhere, inside the shared prefix too.  Keys of an
+ * unmapped page are not visible, as in fpkv_decode_attn.
+ * Takes 16-bit pools in the uniform layout with page_size 128, head_dim 64 or
+ * 128 and at most 16 query heads per stored head (FPKV_ESHAPE / FPKV_EDTYPE
+ * otherwise); n_groups <= FPKV_MAX_GROUPS.
+ * workspace: device, 16-byte aligned, at least fpkv_decode_shared_workspace_bytes()
+ * bytes, of any content; two calls that share one must not overlap.
+ */
+#define FPKV_MAX_GROUPS 1024
+FPKV_API int fpkv_decode_shared_workspace_bytes(const fpkv_pool* pool, int32_t B, int32_t n_q_heads,
+                                                int32_t n_groups, size_t* bytes);
+FPKV_API int fpkv_decode_attn_shared(const fpkv_pool* pool, int32_t layer,
+                                     void* out, float* lse,
+                                     const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                     const int64_t* batch_idx, const void* input_pos, int32_t pos_type,
+                                     int32_t B, int32_t n_q_heads,
+                                     const int32_t* groups, int32_t n_groups, const int32_t* row_group,
+                                     float sm_scale, void* workspace, size_t workspace_bytes,
+                                     const fpkv_epilogue* epilogue, int32_t* status, void* stream);
+
+/*
+ * Indices of one step's packed row, block tables and slot maps from request
+ * lengths that live on the device.  Replaces, for device-held lengths, the host
+ * side of the reference's prefill packing (paged_inference.py:634-678).
+ * Request r brings tokens [starts[r], starts[r] + lens[r]) of slot slots[r]; its
+ * tokens begin at the next multiple of `align` of the packed row, gaps and the
+ * row's end are pads (token pad_id, position 0, slot 0, pool row -1).
+ *   slots   device int64 [n_req];  starts, lens  device int32 [n_req]
+ *   tokens  device int64 [n_tokens], the requests' token ids back to back (read
+ *           only when input_ids is asked for)
+ * Outputs (device; any of them NULL: not written):
+ *   input_ids, input_pos, batch_idx  int64 [row_tokens]
+ *   pool_row     int64 [row_tokens]  page * page_size + position % page_size, the
+ *                token's row in every plane of the pool; -1 for pads and where no
+ *                page is mapped
+ *   block_table  int32 [n_req][width]  physical page of each logical page up to
+ *                the end of the request's tokens, -1 beyond and where unmapped
+ *   seq_lens     int32 [n_req]   starts + lens
+ *   offsets      int32 [n_req+1] packed index of every request's first token, and
+ *                the end of the last one's aligned run
+ *   last         int32 [n_req]   packed index of the last token, -1 without tokens
+ * A request of slot 0 is padding: its tokens are pads.  A negative length or
+ * start counts as a request without tokens and raises FPKV_STATUS_BAD_POS, as do
+ * tokens that do not fit row_tokens (dropped), positions beyond the page table
+ * and a tokens array that is too short (pad_id); a slot out of range raises
+ * FPKV_STATUS_BAD_SLOT (its tokens are pads), a live token without a page
+ * FPKV_STATUS_BAD_PAGE.  n_req <= FPKV_MAX_REQUESTS.
+ */
+#define FPKV_MAX_REQUESTS 4096
+typedef struct fpkv_step_out {
+    int64_t* input_ids;
+    int64_t* input_pos;
+    int64_t* batch_idx;
+    int64_t* pool_row;
+    int32_t* block_table;
+    int32_t* seq_lens;
+    int32_t* offsets;
+    int32_t* last;
+} fpkv_step_out;
+FPKV_API int fpkv_step_tables(const fpkv_pool* pool, const int64_t* slots, const int32_t* starts,
+                              const int32_t* lens, int32_t n_req, int32_t row_tokens, int32_t align,
+                              int32_t width, const int64_t* tokens, int64_t n_tokens, int64_t pad_id,
+                              const fpkv_step_out* out, int32_t* status, void* stream);
+
+/*
+ * One token a row from logits and one given uniform number a row.  Covers the
+ * reference's greedy / temperature / top-k sampling (sampling.py:10-51) and adds
+ * top-p and min-p.  With x the row, max its largest value and T its temperature:
+ *   w_i = exp((x_i - max) / T); entries ordered by x, largest first, ties by
+ *   lowest index; kept: the first top_k of them; of those the shortest leading
+ *   run whose mass reaches top_p of their mass (at least one); of those the
+ *   entries with w_i >= min_p;
+ *   token   = the first kept index, in vocabulary order, at which the running sum
+ *             of the kept w exceeds uniform * their sum;
+ *   logprob = log(w_token / sum of the kept w).
+ * All of this in 64 bits (48 at least), whatever the type of the logits.
+ *   logits       device (rows, vocab) of `dtype`, rows row_stride elements apart,
+ *                vocab contiguous; aligned to its element size
+ *   uniform      device float [rows], in [0, 1)
+ *   temperature  device float [rows] or NULL (1).  <= 0 or NaN: greedy, logprob 0
+ *   top_k        device int32 [rows] or NULL.  <= 0: no limit
+ *   top_p        device float [rows] or NULL.  >= 1 or NaN: no limit; <= 0: one entry
+ *   min_p        device float [rows] or NULL.  <= 0 or NaN: no limit; > 1 counts as 1
+ *   token        device int64 [rows];  logprob  device float [rows] or NULL
+ * A NaN logit counts as -inf; entries of -inf are never drawn; a row with
+ * nothing else gives token -1, logprob -inf.  Entries of +inf share the mass.
+ * vocab <= 2^24.
+ */
+FPKV_API int fpkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
+                         const float* uniform, const float* temperature, const int32_t* top_k,
+                         const float* top_p, const float* min_p, int64_t* token, float* logprob, void* stream);
 
 #ifdef __cplusplus
 }

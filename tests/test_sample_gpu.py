@@ -1,0 +1,213 @@
+"""GPU: token sampling against a 64-bit computation on the host."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from fpkv.sampling import sample
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def reference(logits, u, T=None, k=None, p=None, mp=None):
+    x = logits.detach().double().cpu().numpy()
+    toks, lps = [], []
+    for b, row in enumerate(x):
+        row = np.where(np.isnan(row), -np.inf, row)
+        t = 1.0 if T is None else float(T[b])
+        if row.max() == -np.inf:
+            toks.append(-1); lps.append(-math.inf); continue
+        if not t > 0:
+            toks.append(int(row.argmax())); lps.append(0.0); continue
+        order = np.argsort(-row, kind="stable")
+        order = order[row[order] > -np.inf]
+        if k is not None and int(k[b]) > 0:
+            order = order[:int(k[b])]
+        top = row[order[0]]
+        w = np.where(row == top, 1.0, np.exp((np.where(np.isinf(row), -np.inf, row) - (top if np.isfinite(top) else 0.0)) / t))
+        if not np.isfinite(top):
+            w = (row == top).astype(float)
+        n, ws = len(order), w[order]
+        if p is not None and float(p[b]) < 1:
+            before = np.concatenate([[0.0], np.cumsum(ws)[:-1]])
+            n = max(1, int(np.count_nonzero(before < float(p[b]) * np.cumsum(ws)[-1])))
+        if mp is not None and float(mp[b]) > 0:
+            n = min(n, int(np.count_nonzero(ws >= min(float(mp[b]), 1.0))))
+        ids = np.sort(order[:n])
+        c = np.cumsum(w[ids])
+        j = int(np.searchsorted(c, float(u[b]) * c[-1], side="right"))
+        if j >= n:
+            j = int(np.nonzero(w[ids])[0][-1])
+        toks.append(int(ids[j])); lps.append(math.log(w[ids][j] / c[-1]))
+    return np.array(toks), np.array(lps)
+
+
+def check(logits, u, T=None, k=None, p=None, mp=None, what=""):
+    tok, lp = sample(logits, u, T, k, p, mp)
+    r_tok, r_lp = reference(logits, u, T, k, p, mp)
+    got = tok.cpu().numpy()
+    assert tok.dtype == torch.int64 and lp.dtype == torch.float32
+    assert (got == r_tok).all(), f"{what}: rows {np.nonzero(got != r_tok)[0][:8]}: {got[got != r_tok][:8]} for {r_tok[got != r_tok][:8]}"
+    lp = lp.double().cpu().numpy()
+    fin = np.isfinite(r_lp)
+    assert (np.isfinite(lp) == fin).all() and (lp[~fin] == r_lp[~fin]).all()
+    # 64-bit sums rounded once to 32 bits
+    lp, r_lp = lp[fin], r_lp[fin]
+    assert (np.abs(lp - r_lp) <= 2.0 ** -24 * np.abs(r_lp) + 1e-12).all(), what
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def logits_of(B, V, dtype, g, spread=2.5, masked=0.0):
+    x = torch.randn(B, V, generator=g, device="cuda") * spread
+    if masked:
+        x.masked_fill_(torch.rand(B, V, generator=g, device="cuda") < masked, -math.inf)
+    return x.to(dtype)
+
+
+SETTINGS = {"none": "", "T": "t", "k": "tk", "p": "tp", "min-p": "tm", "all": "tkpm", "greedy-rows": "gkpm"}
+
+
+@pytest.mark.parametrize("setting", SETTINGS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 2), (5, 31), (2, 32), (7, 257), (4, 1000), (3, 4099), (33, 8192), (2, 50001), (1, 131072),
+                                   (2, 262145)], ids=lambda s: f"{s[0]}x{s[1]}")
+def test_against_64_bits(shape, dtype, setting):
+    B, V = shape
+    g = gen(B * 7 + V)
+    for spread, masked in ((2.5, 0.0), (0.05, 0.0), (12.0, 0.4)):
+        x = logits_of(B, V, dtype, g, spread, masked)
+        r = torch.rand(5, B, generator=g, device="cuda")
+        s = SETTINGS[setting]
+        T = 0.2 + 1.5 * r[1] if "t" in s or "g" in s else None
+        if "g" in s:
+            T[::2] = 0.0
+        check(x, r[0].contiguous(), T, (1 + V * r[2] * 0.6).to(torch.int32) if "k" in s else None, r[3].contiguous() if "p" in s else None,
+              0.2 * r[4] if "m" in s else None, f"spread {spread}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+def test_ties(dtype):
+    """Few distinct values: which of the equal entries are kept goes by their index."""
+    g = gen(1)
+    for V in (64, 999, 20000):
+        x = torch.randint(-2, 3, (16, V), generator=g, device="cuda").to(dtype)
+        x[3] = 1.5
+        x[4, ::2] = -0.0; x[4, 1::2] = 0.0               # one value, two bit patterns
+        u = torch.rand(16, generator=g, device="cuda")
+        k = torch.randint(1, V, (16,), generator=g, device="cuda", dtype=torch.int32)
+        p = torch.rand(16, generator=g, device="cuda")
+        check(x, u, k=k); check(x, u, p=p); check(x, u, k=k, p=p)
+
+
+def test_equal_logits_have_exact_borders():
+    """Weights of 1: all sums are whole numbers, borders are hit exactly."""
+    x = torch.full((8, 64), 3.25, dtype=torch.bfloat16, device="cuda")
+    u = torch.arange(8, device="cuda") / 8
+    p = torch.tensor([0.5] * 8, device="cuda")
+    assert sample(x, u, top_p=p)[0].tolist() == [4 * i for i in range(8)]           # 32 kept, u * 32
+    assert sample(x, u, top_k=16, top_p=p)[0].tolist() == list(range(8))            # 8 of the 16 kept
+    assert sample(x, u)[0].tolist() == [8 * i for i in range(8)]
+    assert sample(x, u, min_p=1.0)[0].tolist() == [8 * i for i in range(8)]
+    assert torch.equal(sample(x, u, top_k=8)[1], torch.full((8,), math.log(1 / 8), device="cuda"))
+
+
+def test_extreme_settings():
+    g = gen(3)
+    x = logits_of(12, 5000, torch.float32, g)
+    u = torch.rand(12, generator=g, device="cuda")
+    full = lambda v: torch.full((12,), v, device="cuda")
+    for T in (1e-30, 1e-3, 1e4, math.inf, 0.0, -1.0, math.nan):
+        check(x, u, full(T), what=f"T {T}")
+        check(x, u, full(T), k=torch.full((12,), 7, dtype=torch.int32, device="cuda"), p=full(0.9), mp=full(0.1), what=f"T {T}, filters")
+    for p in (0.0, -1.0, 1e-9, 1 - 2.0 ** -24, 1.0, 2.0, math.nan):
+        check(x, u, p=full(p), what=f"p {p}")
+    for mp in (0.0, -1.0, 1e-30, 1.0, 3.0, math.nan):
+        check(x, u, mp=full(mp), what=f"min_p {mp}")
+    for k in (-5, 0, 1, 4999, 5000, 5001, 2 ** 31 - 1):
+        check(x, u, k=torch.full((12,), k, dtype=torch.int32, device="cuda"), what=f"k {k}")
+    assert torch.equal(sample(x, u, top_k=torch.full((12,), 2 ** 40, device="cuda"))[0], sample(x, u)[0])
+    for uv in (0.0, 1 - 2.0 ** -24, 1.0):
+        check(x, full(uv), what=f"u {uv}"); check(x, full(uv), p=full(0.7), what=f"u {uv}")
+        check(x, full(uv), full(0.01), what=f"u {uv}, cold")      # most weights underflow: the last one that does not
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+def test_masked_and_special_values(dtype):
+    V = 3000
+    g = gen(4)
+    x = logits_of(10, V, dtype, g)
+    low = torch.finfo(dtype).min
+    x[0] = -math.inf                                     # nothing to draw
+    x[1] = math.nan                                      # nothing either
+    x[2] = -math.inf; x[2, 2999] = -5.0                  # one entry, the last
+    x[3] = low; x[3, 17] = 0.0                           # masked by the type's lowest value
+    x[4] = low                                           # all of it
+    x[5, ::3] = math.nan
+    x[6, 100] = math.inf; x[6, 2000] = math.inf          # these two share the mass
+    x[7, :2990] = -math.inf
+    x[8] = torch.finfo(dtype).smallest_normal / 4; x[8, 5] = 0.0; x[8, 6] = -torch.finfo(dtype).smallest_normal / 4   # subnormal values keep their order
+    x[9, 1:] = -math.inf
+    u = torch.rand(10, generator=g, device="cuda")
+    k = torch.tensor([5] * 8 + [2999] + [5], dtype=torch.int32, device="cuda")
+    for kw in ({}, {"k": k}, {"p": torch.full((10,), 0.8, device="cuda")}, {"mp": torch.full((10,), 0.3, device="cuda")},
+               {"T": torch.tensor([0.0, 1.0] * 5, device="cuda")}, {"k": k, "p": torch.full((10,), 0.8, device="cuda")}):
+        check(x, u, what=str(kw.keys()), **kw)
+    tok, lp = sample(x, u)
+    assert tok[:2].tolist() == [-1, -1] and lp[:2].tolist() == [-math.inf, -math.inf]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("V", [40, 1001, 12345, 65536])
+def test_strides_and_alignment(dtype, V):
+    g = gen(V)
+    big = logits_of(6, 2 * V + 8, dtype, g)
+    u = torch.rand(6, generator=g, device="cuda")
+    r = torch.rand(6, generator=g, device="cuda")
+    for at in (0, 1, 3, 8):                              # rows that start anywhere on an element
+        check(big[:, at:at + V], u, p=r)
+    check(big[:, ::2][:, :V], u, p=r)                    # not contiguous: copied
+    check(big[0:1, :V].expand(6, V), u, p=r)             # one row for all
+    check(big[::2, :V], u[::2], p=r[::2])
+
+
+def test_frequencies_follow_the_distribution():
+    """Evenly spaced uniform numbers hit every entry as often as its probability says, to within one."""
+    g = gen(9)
+    x = logits_of(1, 300, torch.bfloat16, g)
+    n = 4096
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    tok, lp = sample(x.expand(n, 300), u.float(), temperature=0.8, top_k=50)
+    count = torch.bincount(tok, minlength=300).double().cpu()
+    keep = torch.topk(x[0].double(), 50).values[-1]
+    prob = torch.softmax(torch.where(x[0].double() >= keep, x[0].double() / float(np.float32(0.8)), -math.inf), 0).cpu()
+    assert (x[0].double() >= keep).sum() >= 50
+    if (x[0].double() >= keep).sum() == 50:
+        assert ((count - n * prob).abs() <= 1 + 1e-6).all()
+    assert (torch.exp(lp.double()).cpu() - count[tok.cpu()] / n).abs().max() <= 2 / n
+
+
+def test_captured_with_new_inputs():
+    g = gen(11)
+    x, u = logits_of(16, 32000, torch.bfloat16, g), torch.rand(16, generator=g, device="cuda")
+    p, k = torch.full((16,), 0.9, device="cuda"), torch.full((16,), 100, dtype=torch.int32, device="cuda")
+    sample(x, u, top_p=p, top_k=k)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tok, lp = sample(x, u, top_p=p, top_k=k)
+    for seed in (1, 2):
+        x.copy_(logits_of(16, 32000, torch.bfloat16, gen(seed))); u.copy_(torch.rand(16, generator=gen(seed + 9), device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_lp = reference(x, u, None, k, p)
+        assert (tok.cpu().numpy() == want).all() and np.allclose(lp.cpu().numpy(), want_lp, rtol=1e-6, atol=1e-9)
+
+
+def test_no_rows():
+    tok, lp = sample(torch.zeros(0, 100, device="cuda"), torch.zeros(0, device="cuda"))
+    assert tok.shape == (0,) and lp.shape == (0,)
