@@ -58,12 +58,9 @@ struct SampleParams {
 // subnormal values keep their order.
 __device__ __forceinline__ uint32_t key_of(uint32_t bits) { return bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u); }
 __device__ __forceinline__ uint32_t bits_of(uint32_t key) { return (key & 0x80000000u) ? (key ^ 0x80000000u) : ~key; }
-// The value in 64 bits, put together from its bits (the conversion unit is a quarter as wide as the 64-bit pipe).
+// The value in 64 bits, put together from its bits (the conversion unit is a quarter as wide as the 64-bit pipe).  Zero and
+// subnormal values come out up to 2^-126 off, which is nothing next to any other value or temperature.
 __device__ __forceinline__ double value_of(uint32_t u) {
-    if ((u & 0x7f800000u) == 0) {                        // zero and subnormal values
-        const double m = (double)(int)(u & 0x007fffffu) * 0x1p-149;
-        return (u >> 31) ? -m : m;
-    }
     return __hiloint2double((int)((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(u << 29));
 }
 
@@ -140,7 +137,7 @@ struct __align__(16) Shared {
     uint32_t pub_low, pub_bound, pub_n, pub_ties;
     uint32_t red_u[kWarps], red_v[kWarps];
     uint32_t n_list;
-    int at[8];
+    int at[16];
 };
 
 template <typename V> __device__ __forceinline__ V warp_sum(V v) {
@@ -350,14 +347,20 @@ sample_kernel(const SampleParams prm)
         s = fma(s, r, 0.6931471805599453094);
         s = fma(s, r, 1.0);
         const double w = s * sh.exp_table[n & 15];
-        if (hi >= 0xC08FF000u)                           // y <= -1022: subnormal or zero
-            return y > -1076.0 ? __hiloint2double(__double2hiint(w) + (((n >> 4) + 1000) << 20), __double2loint(w)) * 0x1p-1000 : 0.0;
-        return __hiloint2double(__double2hiint(w) + ((n >> 4) << 20), __double2loint(w));
+        // no branch, so that several entries' chains overlap: 2^n in two factors, the second one below 1 for subnormal weights
+        const int e = n >> 4, e1 = max(e, -1000);
+        const double scaled = __hiloint2double(__double2hiint(w) + (e1 << 20), __double2loint(w)) * __hiloint2double((1023 + max(e - e1, -90)) << 20, 0);
+        return hi >= 0xC0910000u ? 0.0 : scaled;         // y <= -1088, or no number at all
     };
     // Smallest image at which `holds` is true, which it stays for all larger ones; kmax + 1 if for none.  The lanes of each
     // warp probe 32 places at a time.
-    auto first_key = [&](auto holds) -> uint32_t {
+    // Looked for between near_lo and near_hi first.
+    auto first_key = [&](auto holds, uint32_t near_lo, uint32_t near_hi) -> uint32_t {
         uint32_t lo = kKeyNone + 1u, hi = kmax + 1u;     // the answer is in [lo, hi]
+        if (near_lo >= lo && near_hi < hi && near_lo < near_hi) {
+            const uint32_t yes = __ballot_sync(0xffffffffu, holds(lane == 0 ? near_lo : near_hi));
+            if ((yes & 3u) == 2u) { lo = near_lo + 1u; hi = near_hi; }
+        }
         while (lo < hi) {
             const uint32_t step = (hi - lo) / 32u + 1u, at = lo + (uint32_t)lane * step;
             const uint32_t yes = __ballot_sync(0xffffffffu, at < hi ? holds(at) : true);
@@ -369,28 +372,37 @@ sample_kernel(const SampleParams prm)
     };
     // smallest image that min_p keeps
     const double least = fmin((double)p_min, 1.0);
-    const uint32_t k_least = p_min > 0.f ? first_key([&](uint32_t key) { return weight(bits_of(key)) >= least; }) : 0u;
+    const uint32_t k_least = p_min > 0.f ? first_key([&](uint32_t key) { return weight(bits_of(key)) >= least; }, 0u, 0u) : 0u;
     const unsigned long long n_least = (unsigned long long)k_least << 32;
     const bool by_k = k_top > 0 && k_top < V, by_p = p_top < 1.f;
 
     // ---- bins go by the distance from the maximum in 32 bits, which does not decrease as the value falls ------------
     const float fmx = __uint_as_float(bits_of(kmax)), fslope = (float)slope;
     auto distance = [&](uint32_t bits) { return key_of(bits) == kmax ? 0.f : fminf(fmx - __uint_as_float(bits), 3e38f); };
-    float start = 0.f, per = 0.f;                        // fine bin of a distance: floor((distance - start) * per)
-    auto fine_of = [&](uint32_t bits) -> int {           // -1: before the bins, kFine: behind them
-        const float d = distance(bits);
-        if (d < start) return -1;
-        const float b = (d - start) * per;
-        return b < (float)kFine ? (int)b : kFine;
+    // Images around the value at a distance from the maximum, a few roundings to either side.
+    auto near = [&](float d, bool above) {
+        const float x_ = fmx - d, slack = 4e-7f * (fabsf(fmx) + d);
+        return key_of(__float_as_uint(above ? x_ + slack : x_ - slack));
     };
-    uint32_t k_first = 0, k_last = 0;                    // the images that lie in the fine bins: [k_first, k_last]
-    // smallest image whose fine bin is at most b
-    auto edge = [&](int b) { return first_key([&](uint32_t key) { return fine_of(bits_of(key)) <= b; }); };
-    auto span = [&](float from_, float to) {             // fine bins over [from_, to]
-        start = from_;
-        per = (float)kFine * 0.999f / fmaxf(to - from_, 1e-30f);
-        k_first = edge(kFine - 1);
-        k_last = from_ > 0.f ? edge(-1) - 1u : kmax;
+    // Fine bins: the images in [k_first, k_last], even in the distance; -1 above them, kFine below.
+    uint32_t k_first = 0, k_last = 0;
+    float start = 0.f, per = 0.f;
+    auto span = [&](uint32_t first, uint32_t last) {
+        k_first = first; k_last = last;
+        start = distance(bits_of(last));
+        per = (float)kFine * 0.999f / fmaxf(distance(bits_of(first)) - start, 1e-30f);
+    };
+    auto fine_of = [&](uint32_t key) -> int {
+        if (key > k_last) return -1;
+        if (key < k_first) return kFine;
+        return max(0, min((int)((distance(bits_of(key)) - start) * per), kFine - 1));
+    };
+    // Smallest image whose fine bin is at most b.
+    auto edge = [&](int b) -> uint32_t {
+        if (b < 0) return k_last + 1u;
+        if (b >= kFine - 1) return b < kFine ? k_first : 0u;
+        const float d = start + (float)(b + 1) / per;
+        return first_key([&](uint32_t key) { return fine_of(key) <= b; }, near(d, false), near(d, true));
     };
     auto collect = [&](unsigned long long n) {
         const uint32_t slot = atomicAdd(&sh.n_list, 1u);
@@ -453,12 +465,15 @@ sample_kernel(const SampleParams prm)
         cluster_sync();
         return over_cluster(&sh.pub_d[3]);
     };
-    // Largest number at which `measure`, a sum over the entries at or above it, has `reached` the goal (`lo` if none).
-    auto bisect = [&](unsigned long long lo, auto measure, auto reached) -> unsigned long long {
-        unsigned long long hi = best;
+    // Largest image at which `measure`, a sum over the entries at or above it, reaches the goal; *above is the sum over the
+    // larger ones.  `lo` reaches it.
+    auto bisect = [&](uint32_t lo, auto measure, double goal_, double* above) -> uint32_t {
+        uint32_t hi = kmax;
+        *above = 0;
         while (lo < hi) {
-            const unsigned long long mid = lo + (hi - lo + 1) / 2;
-            if (reached(cluster_sum(measure(mid)))) lo = mid; else hi = mid - 1;
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            const double m = cluster_sum(measure(mid));
+            if (m >= goal_) lo = mid; else { hi = mid - 1; *above = m; }
         }
         return lo;
     };
@@ -470,7 +485,7 @@ sample_kernel(const SampleParams prm)
         each([&](uint32_t bits, int i) {
             const uint32_t key = key_of(bits);
             if (key < k_first || key > k_last || !at_or_above(key, i, thr)) return;
-            atomicAdd(&sh.hist[fine_of(bits)], 1u);
+            atomicAdd(&sh.hist[fine_of(key)], 1u);
         });
     };
     // Chunks of the slice, a warp each: `f(chunk, bits, index)` for every entry, then `done(chunk)`.
@@ -483,6 +498,14 @@ sample_kernel(const SampleParams prm)
 #pragma unroll
                 for (int e = 0; e < VE; ++e) f(Pc::entry(d, e), i0 + v * VE + e);
             }
+            done(c);
+        }
+    };
+    // The same, a piece at a time: f(chunk, piece, index of its first entry).
+    auto each_piece = [&](auto f, auto done) {
+        for (int c = warp; c < n_chunks; c += kWarps) {
+            const int end = min((c + 1) * prm.chunk_vecs, nv);
+            for (int v = c * prm.chunk_vecs + lane; v < end; v += 32) f(piece(v), i0 + v * VE);
             done(c);
         }
     };
@@ -539,7 +562,7 @@ sample_kernel(const SampleParams prm)
         uint32_t lo = 0xffffffffu, hi = 0;
         each([&](uint32_t bits, int i) {
             const uint32_t key = key_of(bits);
-            if (key >= k_first && key <= k_last && at_or_above(key, i, thr) && fine_of(bits) == b) { lo = min(lo, key); hi = max(hi, key); }
+            if (key >= k_first && key <= k_last && at_or_above(key, i, thr) && fine_of(key) == b) { lo = min(lo, key); hi = max(hi, key); }
         });
         lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) { sh.red_u[warp] = lo; sh.red_v[warp] = hi; }
@@ -559,7 +582,7 @@ sample_kernel(const SampleParams prm)
         const uint32_t k = (uint32_t)k_top;
         // Every thread of the cluster that read anything has an entry at or above `bound`.
         const bool bounded = k <= kThreads * C && bound > kKeyNone;
-        span(0.f, distance(bits_of(bounded ? bound : low)));
+        span(bounded ? bound : low, kmax);
         int j = -1; uint32_t in_j = 0, until_j = 0;
         // The bin of the k-th of what was counted, behind `before` others.
         auto find = [&](uint32_t before) {
@@ -575,7 +598,7 @@ sample_kernel(const SampleParams prm)
         bool all_kept = false, done = false;
         if (bounded && 4 * k <= 3 * kCand) {
             // The k-th largest of the threads' largest values has k entries at or above it, and hardly more: collect those.
-            count([&] { if (top > kKeyNone) atomicAdd(&sh.hist[fine_of(bits_of(top))], 1u); });
+            count([&] { if (top > kKeyNone) atomicAdd(&sh.hist[fine_of(top)], 1u); });
             find(0);
             const uint32_t from_key = edge(j);
             each([&](uint32_t bits, int i) { if (key_of(bits) >= from_key) collect(number(key_of(bits), i)); });
@@ -588,18 +611,17 @@ sample_kernel(const SampleParams prm)
             }
         }
         if (!done) {
-            uint32_t before = 0;                         // entries before the fine bins
+            uint32_t before = 0, one = 0;                // entries before the fine bins; the value that fills bin j
             for (int turn = 0;; ++turn) {
                 count([&] { count_entries(everything); });
                 find(before);
                 if (j < 0) { all_kept = turn == 0; break; }              // fewer than k entries above -inf: no limit
-                if (in_j <= (uint32_t)kCand || turn == 3) break;
-                // Too many in one bin: the bin becomes the range.  What lies before it now, rounding included, is counted (the
-                // sum's barriers also mean that the counts have been read).
-                span(start + (float)j / per, start + (float)(j + 1) / per);
-                uint32_t n = 0;
-                each([&](uint32_t bits, int) { n += key_of(bits) > k_last; });
-                before = (uint32_t)cluster_sum((double)n);
+                if (in_j <= (uint32_t)kCand) break;
+                one = only_value(j, everything);
+                if (one != 0 || turn == 3) break;
+                // too many in one bin, of different values: the bin becomes the range
+                before = until_j;
+                span(edge(j), edge(j - 1) - 1u);
             }
             if (j >= 0 && in_j <= (uint32_t)kCand) {
                 const uint32_t from_key = edge(j), to_key = edge(j - 1);
@@ -610,14 +632,16 @@ sample_kernel(const SampleParams prm)
                 gather();
                 threshold = sh.all[k - until_j - 1];
             } else if (!all_kept) {
-                const uint32_t one = j >= 0 ? only_value(j, everything) : 0u;
                 if (one != 0) threshold = nth_equal(one, k - until_j);
-                else
-                    threshold = bisect(everything, [&](unsigned long long thr) {
+                else {
+                    double above;
+                    const uint32_t key = bisect(kKeyNone + 1u, [&](uint32_t from_) {
                         double m = 0;
-                        each([&](uint32_t bits, int i) { if (at_or_above(key_of(bits), i, thr)) m += 1.0; });
+                        each([&](uint32_t bits, int) { m += key_of(bits) >= from_ ? 1.0 : 0.0; });
                         return m;
-                    }, [&](double m) { return m >= (double)k_top; });
+                    }, (double)k, &above);
+                    threshold = nth_equal(key, k - (uint32_t)above);
+                }
             }
         }
         cluster_sync();                                  // lists and counts have been read
@@ -661,14 +685,14 @@ sample_kernel(const SampleParams prm)
         // that is dropped.
         const float far = fminf(fminf(distance(bits_of(low)), temp * logf(2.f * (float)V / (1.f - p_top))), 1e37f);
         const float per_wide = (float)(kWide - 1) / fmaxf(far, 1e-30f);
+        auto wide_of = [&](uint32_t key) { return (int)fminf(distance(bits_of(key)) * per_wide, (float)(kWide - 1)); };
 #pragma unroll
         for (int b = 0; b < kWide; ++b) sh.wide[b][tid] = 0.f;
         each([&](uint32_t bits, int i) {
             if (!at_or_above(key_of(bits), i, threshold)) return;
             const float d = distance(bits);
             const float w = d > 0.f ? exp2f(-d * fslope) : 1.f;
-            const int b = (int)fminf(d * per_wide, (float)(kWide - 1));
-            sh.wide[b][tid] += w;
+            sh.wide[wide_of(key_of(bits))][tid] += w;
         });
         __syncthreads();
         {   // a warp a bin
@@ -690,22 +714,28 @@ sample_kernel(const SampleParams prm)
         const float upto = warp_scan(mass), goal = fmaxf(p_top, 0.f) * __shfl_sync(0xffffffffu, upto, kWide - 1);
         const uint32_t past = __ballot_sync(0xffffffffu, lane < kWide && upto >= goal);
         const int wb = past ? __ffs(past) - 1 : kWide - 1;
-        float mass_before = __shfl_sync(0xffffffffu, upto - mass, wb);
-        // fine bins over that wide bin
+        float mass_before = __shfl_sync(0xffffffffu, upto - mass, wb);       // weight of everything above it
+        // fine bins over the images of that wide bin and half a bin on either side, where the border may be after all
+        auto at_distance = [&](float d) {                // smallest image at most that far from the maximum
+            return first_key([&](uint32_t key) { return distance(bits_of(key)) <= d; }, near(d, false), near(d, true));
+        };
         const float width = 1.f / per_wide;
-        float lo_d = (float)wb * width, hi_d = wb == kWide - 1 ? distance(bits_of(low)) : (float)(wb + 1) * width;
+        float from_d = (float)wb * width;                // where `mass_before` ends
+        span(wb < kWide - 1 ? at_distance(((float)wb + 1.5f) * width) : low, wb > 0 ? at_distance(((float)wb - 0.5f) * width) - 1u : kmax);
         for (int turn = 0; turn < 4; ++turn) {
-            span(lo_d, hi_d);
             count([&] { count_entries(threshold); });
-            if (tid == 0) { sh.at[0] = sh.at[3] = kFine; sh.at[4] = sh.at[7] = -1; sh.at[6] = 0; }
+            if (tid == 0) { sh.at[0] = sh.at[3] = kFine; sh.at[4] = sh.at[7] = sh.at[8] = sh.at[10] = -1; sh.at[6] = sh.at[9] = sh.at[11] = 0; }
             __syncthreads();
             const float d0 = start + ((float)(2 * tid) + 0.5f) / per, d1 = start + ((float)(2 * tid) + 1.5f) / per;
             const float m0 = c0 ? (float)c0 * exp2f(-d0 * fslope) : 0.f, m1 = c1 ? (float)c1 * exp2f(-d1 * fslope) : 0.f;
             float total;
-            const float m_before = mass_before + block_scan(m0 + m1, reinterpret_cast<float*>(sh.red_u), &total) - m0 - m1;
-            if (c0 && m_before + m0 >= goal) atomicMin(&sh.at[0], 2 * tid);
-            else if (c1 && m_before + m0 + m1 >= goal) atomicMin(&sh.at[0], 2 * tid + 1);
-            if (c0 + c1) atomicMax(&sh.at[4], c1 ? 2 * tid + 1 : 2 * tid);
+            const float extra = block_sum((d0 < from_d ? m0 : 0.f) + (d1 < from_d ? m1 : 0.f), reinterpret_cast<float*>(sh.red_u));
+            const float m_before = mass_before - extra + block_scan(m0 + m1, reinterpret_cast<float*>(sh.red_u), &total) - m0 - m1;
+            // one atomic a warp: hundreds on one address take longer than all the rest of this
+            const int here = c0 && m_before + m0 >= goal ? 2 * tid : c1 && m_before + m0 + m1 >= goal ? 2 * tid + 1 : kFine;
+            const int first_here = __reduce_min_sync(0xffffffffu, here), last_here = __reduce_max_sync(0xffffffffu, c1 ? 2 * tid + 1 : c0 ? 2 * tid : -1);
+            if (lane == 0 && first_here < kFine) atomicMin(&sh.at[0], first_here);
+            if (lane == 0 && last_here >= 0) atomicMax(&sh.at[4], last_here);
             __syncthreads();
             // the border by this count; if the estimates do not reach it, the last bin with entries
             const int j = sh.at[0] < kFine ? sh.at[0] : sh.at[4];
@@ -714,6 +744,8 @@ sample_kernel(const SampleParams prm)
                 const uint32_t b = (j & 1) ? c_before + c0 : c_before;
                 sh.at[1] = (int)b; sh.at[2] = (int)((j & 1) ? c1 : c0);
                 sh.at[5] = __float_as_int((j & 1) ? m_before + m0 : m_before);
+                // which of its neighbours is nearer to the border
+                sh.at[12] = goal - ((j & 1) ? m_before + m0 : m_before) > 0.5f * ((j & 1) ? m1 : m0);
             }
             __syncthreads();
             const int at_j = sh.at[1], in_j = sh.at[2];
@@ -722,17 +754,25 @@ sample_kernel(const SampleParams prm)
             const int a0 = (int)c_before, a1 = a0 + (int)c0, a2 = a1 + (int)c1;
             if (c0 && a1 > first && a0 < last) { atomicMin(&sh.at[3], 2 * tid); atomicMax(&sh.at[7], 2 * tid); atomicAdd(&sh.at[6], (int)c0); }
             if (c1 && a2 > first && a1 < last) { atomicMin(&sh.at[3], 2 * tid + 1); atomicMax(&sh.at[7], 2 * tid + 1); atomicAdd(&sh.at[6], (int)c1); }
+            // the nearest bins with entries on either side
+            if (c0 && a1 == at_j) { sh.at[8] = 2 * tid; sh.at[9] = (int)c0; }
+            if (c1 && a2 == at_j) { sh.at[8] = 2 * tid + 1; sh.at[9] = (int)c1; }
+            if (c0 && a0 == at_j + in_j) { sh.at[10] = 2 * tid; sh.at[11] = (int)c0; }
+            if (c1 && a1 == at_j + in_j) { sh.at[10] = 2 * tid + 1; sh.at[11] = (int)c1; }
             __syncthreads();
             if (sh.at[6] <= kCand) { p_lo = sh.at[3]; p_hi = sh.at[7]; break; }
-            if (in_j <= kCand) { p_lo = p_hi = j; break; }
-            if (turn == 3) {
-                tie = only_value(j, threshold);
-                lost = tie == 0;
+            if (in_j <= kCand) {                         // that bin and, if they fit, those of its nearer neighbour
+                p_lo = p_hi = j;
+                if (!sh.at[12] && sh.at[8] >= 0 && in_j + sh.at[9] <= kCand) p_lo = sh.at[8];
+                if (sh.at[12] && sh.at[10] >= 0 && in_j + sh.at[11] <= kCand) p_hi = sh.at[10];
                 break;
             }
+            tie = only_value(j, threshold);
+            lost = tie == 0 && turn == 3;
+            if (tie != 0 || lost) break;
             mass_before = __int_as_float(sh.at[5]);
-            lo_d = start + (float)j / per; hi_d = start + (float)(j + 1) / per;
-            cluster_sync();                              // the counts have been read
+            from_d = 0.f;
+            span(edge(j), edge(j - 1) - 1u);
         }
     }
 
@@ -740,7 +780,19 @@ sample_kernel(const SampleParams prm)
     // chunk by chunk: the sums of what is surely kept stay per chunk, in the order of the vocabulary
     auto sum_chunks = [&](unsigned long long thr) {      // kept: at or above thr
         double kept = 0;
-        each_chunk([&](uint32_t bits, int i) { if (at_or_above(key_of(bits), i, thr)) kept += weight(bits); }, [&](int c) {
+        each_piece([&](const uint4& d, int i) {
+#pragma unroll
+            for (int g = 0; g < VE; g += 4) {            // four chains of dependent 64-bit operations at a time
+                double w[4];
+                bool in[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) in[e] = at_or_above(key_of(Pc::entry(d, g + e)), i + g + e, thr);
+                if (!(in[0] | in[1] | in[2] | in[3])) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { const double y = weight(Pc::entry(d, g + e)); w[e] = in[e] ? y : 0.0; }
+                kept += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+        }, [&](int c) {
             kept = warp_sum(kept);
             if (lane == 0) { sh.chunk_sum[c] = kept; sh.chunk_extra[c] = 0; }
             kept = 0;
@@ -755,22 +807,39 @@ sample_kernel(const SampleParams prm)
         const uint32_t k_sure = lost ? 0u : tie != 0 ? tie + 1u : edge(p_lo - 1);
         const uint32_t k_coll = lost ? 0u : tie != 0 ? tie : edge(p_hi);
         const uint32_t k_chunk = max(k_sure, k_least);   // what counts for the chunks
+        const bool split = k_least > k_sure;             // entries that top-p surely keeps and min_p does not
         double m_all = 0, m_mid = 0, m_ties = 0, kept = 0;
-        each_chunk([&](uint32_t bits, int i) {
-            const uint32_t key = key_of(bits);
-            if (!at_or_above(key, i, threshold)) return;
-            const double w = weight(bits);
-            if (key >= k_chunk) kept += w;
-            else {
-                m_all += w;
-                if (key >= k_sure) m_mid += w;           // top-p keeps it, min_p does not
-                else if (key >= k_coll) {
-                    if (tie != 0) m_ties += 1.0; else collect(number(key, i));
+        each_piece([&](const uint4& d, int i) {
+#pragma unroll
+            for (int g = 0; g < VE; g += 4) {
+                double w[4];
+                uint32_t key[4];
+                bool in[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    key[e] = key_of(Pc::entry(d, g + e));
+                    in[e] = at_or_above(key[e], i + g + e, threshold);
                 }
+                if (!(in[0] | in[1] | in[2] | in[3])) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { const double y = weight(Pc::entry(d, g + e)); w[e] = in[e] ? y : 0.0; }
+                m_all += (w[0] + w[1]) + (w[2] + w[3]);
+                if (split) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (key[e] >= k_sure) m_mid += w[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (key[e] < k_sure && key[e] >= k_coll && in[e]) {
+                        if (tie != 0) m_ties += 1.0; else collect(number(key[e], i + g + e));
+                    }
+                    w[e] = key[e] >= k_chunk ? w[e] : 0.0;
+                }
+                kept += (w[0] + w[1]) + (w[2] + w[3]);
             }
         }, [&](int c) {
             kept = warp_sum(kept);
-            if (lane == 0) { sh.chunk_sum[c] = kept; sh.chunk_extra[c] = 0; m_all += kept; m_mid += kept; }
+            if (lane == 0) { sh.chunk_sum[c] = kept; sh.chunk_extra[c] = 0; if (!split) m_mid += kept; }
             kept = 0;
         });
         block_sum3(m_all, m_mid, m_ties, sh.red_d);
@@ -778,14 +847,18 @@ sample_kernel(const SampleParams prm)
         const int n = gather();
         const double M = over_cluster(&sh.pub_d[0]), A = over_cluster(&sh.pub_d[1]);
         const double goal = (double)p_top * M;
+        // entries of weight w from above on: as many as start below the goal, at least one
+        auto taken = [&](double above, double w, double many) {
+            double take = fmin(fmax(ceil((goal - above) / w), 1.0), many);
+            while (take > 1.0 && above + (take - 1.0) * w >= goal) take -= 1.0;
+            while (take < many && above + take * w < goal) take += 1.0;
+            return (uint32_t)take;
+        };
         bool right = false;                              // whether the border lies where it was guessed
         if (tie != 0) {
             const double many = over_cluster(&sh.pub_d[2]), w = weight(bits_of(tie));
             if (A < goal && A + many * w >= goal) {
-                double take = fmin(fmax(ceil((goal - A) / w), 1.0), many);
-                while (take > 1.0 && A + (take - 1.0) * w >= goal) take -= 1.0;
-                while (take < many && A + take * w < goal) take += 1.0;
-                threshold = nth_equal(tie, (uint32_t)take);
+                threshold = nth_equal(tie, taken(A, w, many));
                 threshold = threshold > n_least ? threshold : n_least;
                 sum_chunks(threshold);
                 right = true;
@@ -808,11 +881,19 @@ sample_kernel(const SampleParams prm)
             }
         }
         if (!right) {
-            threshold = bisect(threshold, [&](unsigned long long thr) {
+            double above;
+            const uint32_t key = bisect((uint32_t)(threshold >> 32), [&](uint32_t from_) {
                 double m = 0;
-                each([&](uint32_t bits, int i) { if (at_or_above(key_of(bits), i, thr)) m += weight(bits); });
+                each([&](uint32_t bits, int i) {
+                    const uint32_t at = key_of(bits);
+                    if (at >= from_ && at_or_above(at, i, threshold)) m += weight(bits);
+                });
                 return m;
-            }, [&](double m) { return m >= goal; });
+            }, goal, &above);
+            double many = 0;
+            each([&](uint32_t bits, int i) { if (key_of(bits) == key && at_or_above(key, i, threshold)) many += 1.0; });
+            many = cluster_sum(many);
+            threshold = nth_equal(key, taken(above, weight(bits_of(key)), many));
             threshold = threshold > n_least ? threshold : n_least;
             sum_chunks(threshold);
         }
