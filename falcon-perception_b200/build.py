@@ -22,7 +22,7 @@ from fpkv._srchash import CSRC, source_hash  # noqa: E402  (does not load the li
 
 OUT = os.path.join(HERE, "fpkv", "libfpkv.so")
 SOURCES = ["api.cu", "append.cu", "pre_append.cu", "decode_portable.cu", "decode_tma.cu", "decode_static.cu",
-           "decode_shared.cu", "prefill_tc.cu", "tables.cu", "step_tables.cu", "sample.cu"]
+           "decode_shared.cu", "shared_prefix_tc.cu", "prefill_tc.cu", "tables.cu", "step_tables.cu", "sample.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
               "--use_fast_math", "-Xcompiler", "-fPIC,-O3,-fvisibility=hidden", "-shared"]
 

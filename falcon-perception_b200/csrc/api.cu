@@ -302,7 +302,7 @@ static int check_shared(const PoolView& pv, int32_t B, int32_t n_q_heads, int32_
     if (B < 0 || n_q_heads <= 0 || n_groups < 0) return FPKV_EINVAL;
     if (pv.dtype != FPKV_BF16 && pv.dtype != FPKV_F16) return FPKV_EDTYPE;
     if (n_q_heads % pv.H || n_groups > FPKV_MAX_GROUPS || !decode_shared_supported(pv, n_q_heads)) return FPKV_ESHAPE;
-    // grids are B * n_q_heads blocks wide and positions are 32-bit on the device
+    // grids are B * n_q_heads blocks wide and key positions are 32-bit on the device
     if ((long long)B * n_q_heads > (1ll << 24) || (long long)pv.n_pages * pv.P >= (1ll << 31)) return FPKV_ESHAPE;
     return FPKV_OK;
 }
@@ -329,7 +329,7 @@ int fpkv_decode_attn_shared(const fpkv_pool* pool, int32_t layer, void* out, flo
     if (rc) return rc;
     Epilogue epi;
     if ((rc = make_epilogue(epilogue, n_q_heads, &epi))) return rc;
-    if (pos_type != FPKV_I32 && pos_type != FPKV_I64) return FPKV_EINVAL;
+    if ((pos_type != FPKV_I32 && pos_type != FPKV_I64) || !(sm_scale > 0.f)) return FPKV_EINVAL;
     if ((rc = check_shared(pv, B, n_q_heads, n_groups))) return rc;
     if (B == 0) return FPKV_OK;
     if (out == nullptr || lse == nullptr || batch_idx == nullptr || input_pos == nullptr || workspace == nullptr)

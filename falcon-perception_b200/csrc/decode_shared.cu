@@ -3,76 +3,50 @@
 // With keys 0 .. s-1 the same for every row of a group, the softmax over a row's keys splits into the prefix part and
 // the row's own part, each with its own maximum m, sum l and unnormalised result a (all in 32 bits):
 //     M = max(m1, m2),  l = l1 2^(m1-M) + l2 2^(m2-M),  out = (a1 2^(m1-M) + a2 2^(m2-M)) / l
-// (scores in base 2).  The prefix part of all rows of a group is one pass over the prefix's keys, so they are read
-// once a group instead of once a row.
+// (scores in base 2).  The prefix part of all rows of a group is one product over the prefix's keys, so they are read
+// once a group instead of once a row.  Three launches:
 //
-//  * partial kernel: a CTA takes a tile of up to 16 query rows of one stored head -- the GQA group of one batch row over
-//    that row's own keys, or the GQA groups of several rows over their common prefix -- and a share of the keys.  Its
-//    warps walk blocks of 16 keys; K and V go from memory straight into the registers of mma.sync.m16n8k16: the order of
-//    the contraction index and of the output columns is free, so it is chosen such that every lane's 16-byte piece of a
-//    row is its own operand.  No shared memory, no barrier in the loop.
-//  * merge kernel: joins the partials of every (row, head), applies the sink gate, writes out and lse.
+//  * prefix part: shared_prefix_tc.cu.
+//  * own part, below: a CTA takes the query heads of one stored head of one batch row (up to 16, the M rows of
+//    mma.sync.m16n8k16) and a share of the row's keys behind the prefix.  Its warps walk blocks of 16 keys; K and V go
+//    from memory straight into the registers of the MMAs: the order of the contraction index and of the output columns is
+//    free, so it is chosen such that every lane's 16-byte piece of a row is its own operand.  No shared memory, no barrier
+//    in the loop.  Bound by the bytes of the rows' own keys.
+//  * merge: joins the partials of every (row, head), applies the sink gate, writes out and lse.
 
-#include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace fpkv {
 
 namespace {
 
 constexpr int kPage = 128;
-constexpr int kTileRows = 16;                  // query rows of a partial
+constexpr int kMaxRep = 16;                    // query heads of a stored head: rows of the own part's MMAs
 constexpr int kPartWarps = 4;
 constexpr int kListTiles = 64;                 // pages resolved at a time
 
-struct SharedParams {
+struct OwnParams {
+    RowParams rows;
     const char* k;                             // K plane of stored head 0
     const char* v;
     size_t plane_bytes;
-    const int64_t* page_table;
-    const int64_t* p2l;
-    const int64_t* batch_idx;
-    const void* pos;
     const void* q;
-    const int4* groups;                        // {first row, rows, shared pages, 0}
-    const int* row_group;
-    void* out;
-    float* lse;
-    float* ws;                                 // partials [part][16 rows][D + 2]: m, l, a[D]
-    int32_t* status;
+    float2* ml;                                // partials [B][Hq][splits] (m, l)
+    float* acc;                                // [B][Hq][splits][D]
     long long q_stride_b, q_stride_h;
-    int B, Hq, H, n_rep, rows_per_tile, n_groups, n_pages, max_batch, pos_is_64;
-    int prefix_tiles, prefix_splits, own_splits;        // grid: prefix_tiles * H * prefix_splits, then B * H * own_splits
+    int splits;
     float scale_log2;
-    Epilogue epi;
 };
 
-__device__ __forceinline__ long long pos_of(const SharedParams& p, int b) {
-    return p.pos_is_64 ? reinterpret_cast<const int64_t*>(p.pos)[b] : (long long)reinterpret_cast<const int32_t*>(p.pos)[b];
-}
-// Slot and visible keys of a row; a slot or position out of range gives no keys.
-__device__ __forceinline__ int row_keys(const SharedParams& p, int b, int* slot, bool report) {
-    const long long s = p.batch_idx[b], at = pos_of(p, b);
-    *slot = 0;
-    if (s < 0 || s >= p.max_batch) { if (report) raise_status(p.status, FPKV_STATUS_BAD_SLOT); return 0; }
-    if (at < 0 || at / kPage >= p.n_pages) { if (report) raise_status(p.status, FPKV_STATUS_BAD_POS); return 0; }
-    *slot = (int)s;
-    return (int)at + 1;
-}
-// A group as the kernels use it: rows and pages inside the batch and the table, or nothing.
-__device__ __forceinline__ int4 group_at(const SharedParams& p, int g) {
-    int4 d = p.groups[g];
-    if (d.x < 0 || d.y <= 0 || d.x >= p.B || d.y > p.B - d.x || d.z <= 0) d.y = d.z = 0;
-    d.z = min(d.z, p.n_pages);
-    return d;
-}
-__device__ __forceinline__ int tiles_of(const SharedParams& p, const int4& d) { return (d.y + p.rows_per_tile - 1) / p.rows_per_tile; }
-// Group of a row (or -1) and, when asked for, the row's tile number over all groups.
-__device__ __forceinline__ int group_of_row(const SharedParams& p, int b, int4* d) {
-    const int g = p.n_groups > 0 ? p.row_group[b] : -1;
-    if (g < 0 || g >= p.n_groups) return -1;
-    *d = group_at(p, g);
-    return (d->y > 0 && b >= d->x && b < d->x + d->y) ? g : -1;
-}
+struct MergeParams {
+    RowParams rows;
+    const float2* pre_ml; const float* pre_acc;
+    const float2* own_ml; const float* own_acc;
+    int splits, ctas, tiles;                   // of the own part; of the prefix part; upper bound of its query tiles
+    void* out;
+    float* lse;
+    Epilogue epi;
+};
 
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -96,74 +70,32 @@ __device__ __forceinline__ uint4 ld16(const char* p) { return *reinterpret_cast<
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPartWarps * 32)
-shared_partial_kernel(const SharedParams prm)
+own_part_kernel(const OwnParams prm)
 {
     constexpr int NI = D / 32, NH = D / 64;    // 16-byte pieces of a K row per lane; 64-column groups of a V row
+    const RowParams& rp = prm.rows;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
     __shared__ int s_row[kListTiles];          // pool row of each resolved page, -1 = not visible
-    __shared__ float s_m[kPartWarps][kTileRows], s_l[kPartWarps][kTileRows];
-    __shared__ float s_acc[kPartWarps][kTileRows][D + 4];
+    __shared__ float s_m[kPartWarps][kMaxRep], s_l[kPartWarps][kMaxRep];
+    __shared__ float s_acc[kPartWarps][kMaxRep][D + 4];
 
-    // ---- which tile, which keys ---------------------------------------------------
-    const int n_prefix = prm.prefix_tiles * prm.H * prm.prefix_splits;
-    const int id = blockIdx.x;
-    int h, b0, nb, split, splits, first_page, end_page;
-    if (id < n_prefix) {
-        split = id % prm.prefix_splits; splits = prm.prefix_splits;
-        h = (id / prm.prefix_splits) % prm.H;
-        int t = id / (prm.prefix_splits * prm.H);
-        int gr = 0; int4 d = make_int4(0, 0, 0, 0);
-        for (; gr < prm.n_groups; ++gr) {      // tile t of all groups' tiles
-            d = group_at(prm, gr);
-            const int n = tiles_of(prm, d);
-            if (t < n) break;
-            t -= n;
-        }
-        if (gr == prm.n_groups) return;
-        b0 = d.x + t * prm.rows_per_tile;
-        nb = min(prm.rows_per_tile, d.x + d.y - b0);
-        first_page = 0; end_page = d.z;
-    } else {
-        const int k = id - n_prefix;
-        split = k % prm.own_splits; splits = prm.own_splits;
-        h = (k / prm.own_splits) % prm.H;
-        b0 = k / (prm.own_splits * prm.H); nb = 1;
-        int4 d;
-        first_page = group_of_row(prm, b0, &d) >= 0 ? d.z : 0;
-        end_page = prm.n_pages;
-    }
-    // the rows of this tile: lane's rows g and g + 8
-    int keys[2], hi_keys = 0, slot0 = 0;
-    for (int r = 0; r < nb; ++r) {
-        int s; const int n = row_keys(prm, b0 + r, &s, h == 0 && split == 0 && threadIdx.x == 0 && id >= n_prefix);
-        if (r == 0) slot0 = s;
-        hi_keys = max(hi_keys, n);
-    }
-    const int rows = nb * prm.n_rep;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        int s;
-        keys[r] = row < rows ? row_keys(prm, b0 + row / prm.n_rep, &s, false) : 0;
-    }
-    {   // the prefix is read through the first row's slot; a first row out of range leaves the group to no one
-        long long s = prm.batch_idx[b0];
-        slot0 = (s >= 0 && s < prm.max_batch) ? (int)s : 0;
-    }
-    end_page = min(end_page, (hi_keys + kPage - 1) / kPage);
+    const int split = blockIdx.x % prm.splits, h = (blockIdx.x / prm.splits) % rp.H, b0 = blockIdx.x / (prm.splits * rp.H);
+    const int rows = rp.n_rep;
+    int slot0; int4 d;
+    const int hi_keys = row_keys(rp, b0, &slot0, h == 0 && split == 0 && threadIdx.x == 0);
+    const int first_page = group_of_row(rp, b0, &d) >= 0 ? d.z : 0, end_page = (hi_keys + kPage - 1) / kPage;
     const int n_pg = max(0, end_page - first_page);
-    const int pg0 = first_page + (int)((long long)n_pg * split / splits), pg1 = first_page + (int)((long long)n_pg * (split + 1) / splits);
-    const int lim = id < n_prefix ? end_page * kPage : 0x7fffffff;      // keys past the shared pages are the own part's
-    keys[0] = min(keys[0], lim); keys[1] = min(keys[1], lim);
+    const int pg0 = first_page + (int)((long long)n_pg * split / prm.splits), pg1 = first_page + (int)((long long)n_pg * (split + 1) / prm.splits);
+    const int keys[2] = {hi_keys, hi_keys};
 
-    // ---- queries: row g and row g + 8, dims i * 32 + c * 8 .. + 7 --------------------------
+    // queries: rows g and g + 8 of the MMAs, dims i * 32 + c * 8 .. + 7
     uint4 qa[NI], qb[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         qa[i] = qb[i] = make_uint4(0, 0, 0, 0);
         const T* q = reinterpret_cast<const T*>(prm.q);
-        if (g < rows) qa[i] = ld16(reinterpret_cast<const char*>(q + (b0 + g / prm.n_rep) * prm.q_stride_b + (h * prm.n_rep + g % prm.n_rep) * prm.q_stride_h + i * 32 + c * 8));
-        if (g + 8 < rows) qb[i] = ld16(reinterpret_cast<const char*>(q + (b0 + (g + 8) / prm.n_rep) * prm.q_stride_b + (h * prm.n_rep + (g + 8) % prm.n_rep) * prm.q_stride_h + i * 32 + c * 8));
+        if (g < rows) qa[i] = ld16(reinterpret_cast<const char*>(q + b0 * prm.q_stride_b + (h * rows + g) * prm.q_stride_h + i * 32 + c * 8));
+        if (g + 8 < rows) qb[i] = ld16(reinterpret_cast<const char*>(q + b0 * prm.q_stride_b + (h * rows + g + 8) * prm.q_stride_h + i * 32 + c * 8));
     }
     float acc[NH][8][4];
 #pragma unroll
@@ -179,10 +111,10 @@ shared_partial_kernel(const SharedParams prm)
     for (int p0 = pg0; p0 < pg1; p0 += kListTiles) {
         __syncthreads();
         for (int j = threadIdx.x; j < min(kListTiles, pg1 - p0); j += kPartWarps * 32) {
-            const long long pg = prm.page_table[(long long)slot0 * prm.n_pages + p0 + j];
+            const long long pg = rp.page_table[(long long)slot0 * rp.n_pages + p0 + j];
             int row = -1;
-            if (pg >= prm.n_pages) raise_status(prm.status, FPKV_STATUS_BAD_PAGE);
-            else if (pg >= 0 && prm.p2l[(long long)slot0 * prm.n_pages + pg] >= 0) row = (int)pg * kPage;
+            if (pg >= rp.n_pages) raise_status(rp.status, FPKV_STATUS_BAD_PAGE);
+            else if (pg >= 0 && rp.p2l[(long long)slot0 * rp.n_pages + pg] >= 0) row = (int)pg * kPage;
             s_row[j] = row;
         }
         __syncthreads();
@@ -282,66 +214,121 @@ shared_partial_kernel(const SharedParams prm)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s_acc[warp][g + 8 * (k >> 1)][a * 64 + (2 * c + (k & 1)) * 8 + e] = acc[a][e][k];
     __syncthreads();
-    float* dst = prm.ws + (size_t)id * kTileRows * (D + 2);
     for (int i = threadIdx.x; i < rows * D; i += kPartWarps * 32) {
-        const int r = i / D, d = i % D;
+        const int r = i / D, col = i % D;
+        const size_t part = ((size_t)b0 * rp.Hq + h * rows + r) * prm.splits + split;
         float M = -INFINITY;
         for (int w = 0; w < kPartWarps; ++w) M = fmaxf(M, s_m[w][r]);
         float L = 0.f, o = 0.f;
         for (int w = 0; w < kPartWarps; ++w)
-            if (s_m[w][r] != -INFINITY) { const float f = exp2f(s_m[w][r] - M); L += s_l[w][r] * f; o += s_acc[w][r][d] * f; }
-        dst[r * (D + 2) + 2 + d] = o;
-        if (d == 0) { dst[r * (D + 2)] = M; dst[r * (D + 2) + 1] = L; }
+            if (s_m[w][r] != -INFINITY) { const float f = exp2f(s_m[w][r] - M); L += s_l[w][r] * f; o += s_acc[w][r][col] * f; }
+        prm.acc[part * D + col] = o;
+        if (col == 0) prm.ml[part] = make_float2(M, L);
     }
 }
 
+// Columns [4 * col4, +4 * N) of one (row, head): the weighted sum of its partials.
+template <int N> struct Sum {
+    float a[4 * N], L, M;
+    __device__ __forceinline__ void add(float w, const float4* src, size_t step) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float4 v = src[k * step];
+            a[4 * k] += w * v.x; a[4 * k + 1] += w * v.y; a[4 * k + 2] += w * v.z; a[4 * k + 3] += w * v.w;
+        }
+    }
+};
+
+// Block: 32 query rows of a query tile (one stored head), a row a lane, the columns dealt out to the warps; behind those one
+// block for each batch row that is in no group.
 template <typename T, int D>
-__global__ void __launch_bounds__(D)
-shared_merge_kernel(const SharedParams prm)
+__global__ void __launch_bounds__(128)
+shared_merge_kernel(const MergeParams prm)
 {
-    const int b = blockIdx.x / prm.Hq, hq = blockIdx.x % prm.Hq, h = hq / prm.n_rep, rep = hq % prm.n_rep, d = threadIdx.x;
-    const int n_prefix = prm.prefix_tiles * prm.H * prm.prefix_splits;
-    const float* own = prm.ws + ((size_t)n_prefix + ((size_t)b * prm.H + h) * prm.own_splits) * kTileRows * (D + 2) + (size_t)rep * (D + 2);
-    const float* pre = nullptr;
-    int4 gd;
-    const int g = group_of_row(prm, b, &gd);
-    if (g >= 0) {
-        int t = 0;
-        for (int i = 0; i < g; ++i) { const int4 o = group_at(prm, i); t += tiles_of(prm, o); }
-        const int in = b - gd.x;
-        t += in / prm.rows_per_tile;
-        pre = prm.ws + ((size_t)t * prm.H + h) * prm.prefix_splits * kTileRows * (D + 2) +
-              (size_t)((in % prm.rows_per_tile) * prm.n_rep + rep) * (D + 2);
+    constexpr int N = D / 16;                  // column groups of four a warp (a block has four warps)
+    const RowParams& rp = prm.rows;
+    __shared__ long long flat_before[FPKV_MAX_GROUPS + 1];
+    __shared__ int mt_before[FPKV_MAX_GROUPS + 1];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tile_blocks = prm.tiles * rp.H * (kPrefixTileRows / 32);
+    int b, hq, c0 = 0, c1 = -1, index = 0, trow = 0;
+    if ((int)blockIdx.x < tile_blocks) {
+        if (warp == 0) prefix_schedule(rp, flat_before, mt_before, lane);
+        __syncthreads();
+        const int quarter = blockIdx.x % (kPrefixTileRows / 32), seg0 = blockIdx.x / (kPrefixTileRows / 32);
+        if (seg0 >= mt_before[rp.n_groups] * rp.H) return;
+        int lo = 0, hi = rp.n_groups;          // the group whose segments (query tiles times stored heads) hold this one
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (mt_before[mid] * rp.H <= seg0) lo = mid; else hi = mid; }
+        const int4 d = group_at(rp, lo);
+        const Segment sg = segment_at(rp, flat_before, mt_before, flat_before[lo] + (long long)(seg0 - mt_before[lo] * rp.H) * d.z);
+        trow = quarter * 32 + lane;
+        if (quarter * 32 >= sg.rows) return;
+        const long long total = flat_before[rp.n_groups], first = flat_before[lo] + (long long)(seg0 - mt_before[lo] * rp.H) * d.z;
+        const int ctas = sharers(total, prm.ctas);
+        c0 = share_of(total, first, ctas); c1 = share_of(total, first + d.z - 1, ctas);
+        index = sg.index;
+        b = sg.b0 + trow / rp.n_rep; hq = sg.h * rp.n_rep + trow % rp.n_rep;
+        int4 mine;
+        // a row of the tile that does not name the group has all its keys in its own part
+        if (trow >= sg.rows) b = -1;
+        else if (group_of_row(rp, b, &mine) != lo) b = -1;
+    } else {
+        const int i = (blockIdx.x - tile_blocks) * 32 + lane;
+        b = i / rp.Hq; hq = i % rp.Hq;
+        int4 mine;
+        if (b >= rp.B || group_of_row(rp, b, &mine) >= 0) b = -1;
     }
-    const size_t step = (size_t)kTileRows * (D + 2);
-    float M = -INFINITY;
-    for (int s = 0; s < prm.own_splits; ++s) M = fmaxf(M, own[s * step]);
-    if (pre != nullptr) for (int s = 0; s < prm.prefix_splits; ++s) M = fmaxf(M, pre[s * step]);
-    float L = 0.f, o = 0.f;
-    auto add = [&](const float* x) {
-        if (x[0] == -INFINITY) return;
-        const float w = exp2f(x[0] - M);
-        L += x[1] * w; o += x[2 + d] * w;
-    };
-    for (int s = 0; s < prm.own_splits; ++s) add(own + s * step);
-    if (pre != nullptr) for (int s = 0; s < prm.prefix_splits; ++s) add(pre + s * step);
-    const float lse = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
-    reinterpret_cast<T*>(prm.out)[(size_t)blockIdx.x * D + d] =
-        gated_out<T>(L == 0.f ? 0.f : o / L, sink_gate(prm.epi, hq, lse), prm.epi.sinks != nullptr);
-    if (d == 0) prm.lse[blockIdx.x] = lse;
+    if (b < 0) return;
+    const size_t row = (size_t)b * rp.Hq + hq, own = row * prm.splits;
+    Sum<N> s;
+    s.M = -INFINITY; s.L = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4 * N; ++k) s.a[k] = 0.f;
+    for (int c = c0; c <= c1; ++c) s.M = fmaxf(s.M, prm.pre_ml[(size_t)(c + index) * kPrefixTileRows + trow].x);
+    for (int k = 0; k < prm.splits; ++k) s.M = fmaxf(s.M, prm.own_ml[own + k].x);
+    for (int c = c0; c <= c1; ++c) {
+        const float2 ml = prm.pre_ml[(size_t)(c + index) * kPrefixTileRows + trow];
+        if (ml.y == 0.f) continue;             // nothing visible: no sums were written
+        const float w = exp2f(ml.x - s.M);
+        s.L += ml.y * w;
+        s.add(w, reinterpret_cast<const float4*>(prm.pre_acc) + ((size_t)(c + index) * (D / 4) + warp * N) * kPrefixTileRows + trow, kPrefixTileRows);
+    }
+    for (int k = 0; k < prm.splits; ++k) {
+        const float2 ml = prm.own_ml[own + k];
+        if (ml.y == 0.f) continue;
+        const float w = exp2f(ml.x - s.M);
+        s.L += ml.y * w;
+        s.add(w, reinterpret_cast<const float4*>(prm.own_acc) + (own + k) * (D / 4) + warp * N, 1);
+    }
+    const float lse = s.L == 0.f ? -INFINITY : (s.M + log2f(s.L)) * kLn2;
+    const float gate = sink_gate(prm.epi, hq, lse), inv = s.L == 0.f ? 0.f : 1.f / s.L;
+    T o[4 * N];
+#pragma unroll
+    for (int k = 0; k < 4 * N; ++k) o[k] = gated_out<T>(s.a[k] * inv, gate, prm.epi.sinks != nullptr);
+    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(prm.out) + row * D + warp * 4 * N);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) dst[k] = reinterpret_cast<const uint4*>(o)[k];
+    if (warp == 0) prm.lse[row] = lse;
 }
 
-struct Plan { int rows_per_tile, prefix_tiles, prefix_splits, own_splits; size_t parts; };
+struct Plan { int n_rep, rows_per_tile, tiles, splits; size_t slots, pre_ml, pre_acc, own_ml, own_acc, bytes; };
 Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
 {
     Plan p;
-    const int n_rep = Hq / pv.H;
-    p.rows_per_tile = kTileRows / n_rep;
-    p.prefix_tiles = n_groups > 0 ? B / p.rows_per_tile + (n_groups < B ? n_groups : B) : 0;
-    auto splits = [](int tiles) { const int s = tiles > 0 ? 4 * 148 / tiles : 1; return s < 1 ? 1 : s > 32 ? 32 : s; };
-    p.prefix_splits = splits(p.prefix_tiles * pv.H);
-    p.own_splits = splits(B * pv.H);
-    p.parts = (size_t)p.prefix_tiles * pv.H * p.prefix_splits + (size_t)B * pv.H * p.own_splits;
+    p.n_rep = Hq / pv.H;
+    p.rows_per_tile = kPrefixTileRows / p.n_rep;
+    // a group leaves at most one tile that is not full
+    p.tiles = n_groups > 0 ? B / p.rows_per_tile + (n_groups < B ? n_groups : B) : 0;
+    // Own part: four CTAs an SM when there are few rows.
+    p.splits = 4 * 148 / (B * pv.H > 0 ? B * pv.H : 1);
+    p.splits = p.splits < 1 ? 1 : p.splits > 32 ? 32 : p.splits;
+    p.slots = p.tiles > 0 ? (size_t)p.tiles * pv.H + prefix_ctas() : 0;
+    auto place = [at = (size_t)0](size_t n) mutable { const size_t was = at; at += (n + 255) / 256 * 256; return was; };
+    p.pre_ml = place(p.slots * kPrefixTileRows * sizeof(float2));
+    p.pre_acc = place(p.slots * kPrefixTileRows * pv.D * sizeof(float));
+    p.own_ml = place((size_t)B * Hq * p.splits * sizeof(float2));
+    p.own_acc = place((size_t)B * Hq * p.splits * pv.D * sizeof(float));
+    p.bytes = place(0);
     return p;
 }
 
@@ -349,13 +336,10 @@ Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
 
 bool decode_shared_supported(const PoolView& pv, int Hq)
 {
-    return (pv.dtype == FPKV_BF16 || pv.dtype == FPKV_F16) && pv.split_hq == 0 && pv.P == kPage && Hq / pv.H <= kTileRows;
+    return (pv.dtype == FPKV_BF16 || pv.dtype == FPKV_F16) && pv.split_hq == 0 && pv.P == kPage && Hq / pv.H <= kMaxRep && prefix_supported(pv);
 }
 
-size_t decode_shared_workspace_bytes(const PoolView& pv, int B, int Hq, int n_groups)
-{
-    return plan_of(pv, B, Hq, n_groups).parts * kTileRows * (pv.D + 2) * sizeof(float);
-}
+size_t decode_shared_workspace_bytes(const PoolView& pv, int B, int Hq, int n_groups) { return plan_of(pv, B, Hq, n_groups).bytes; }
 
 int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, const void* q, long long qsb, long long qsh,
                          const int64_t* batch_idx, const void* pos, int pos_type, int B, int Hq, const int32_t* groups,
@@ -363,27 +347,38 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
                          int32_t* status, cudaStream_t stream)
 {
     const Plan pl = plan_of(pv, B, Hq, n_groups);
-    SharedParams prm;
-    prm.k = pv.plane(layer, 0, 0); prm.v = pv.plane(layer, 1, 0); prm.plane_bytes = pv.plane_bytes();
-    prm.page_table = pv.page_table; prm.p2l = pv.p2l; prm.batch_idx = batch_idx; prm.pos = pos; prm.q = q;
-    prm.groups = reinterpret_cast<const int4*>(groups); prm.row_group = row_group;
-    prm.out = out; prm.lse = lse; prm.ws = static_cast<float*>(workspace); prm.status = status;
-    prm.q_stride_b = qsb; prm.q_stride_h = qsh;
-    prm.B = B; prm.Hq = Hq; prm.H = pv.H; prm.n_rep = Hq / pv.H; prm.rows_per_tile = pl.rows_per_tile;
-    prm.n_groups = n_groups; prm.n_pages = pv.n_pages; prm.max_batch = pv.max_batch; prm.pos_is_64 = pos_type == FPKV_I64;
-    prm.prefix_tiles = pl.prefix_tiles; prm.prefix_splits = pl.prefix_splits; prm.own_splits = pl.own_splits;
-    prm.scale_log2 = sm_scale * kLog2e; prm.epi = epi;
+    char* ws = static_cast<char*>(workspace);
+    RowParams rows;
+    rows.page_table = pv.page_table; rows.p2l = pv.p2l; rows.batch_idx = batch_idx; rows.pos = pos;
+    rows.groups = reinterpret_cast<const int4*>(groups); rows.row_group = row_group; rows.status = status;
+    rows.B = B; rows.Hq = Hq; rows.H = pv.H; rows.n_rep = pl.n_rep; rows.n_groups = n_groups; rows.n_pages = pv.n_pages;
+    rows.max_batch = pv.max_batch; rows.pos_is_64 = pos_type == FPKV_I64; rows.rows_per_tile = pl.rows_per_tile;
+    if (n_groups > 0) {
+        PrefixParams pre;
+        pre.rows = rows; pre.ml = reinterpret_cast<float2*>(ws + pl.pre_ml); pre.acc = reinterpret_cast<float*>(ws + pl.pre_acc);
+        pre.rows_per_plane = 0; pre.q_box_rows = 0; pre.scale_log2 = sm_scale * kLog2e;
+        const int rc = launch_prefix(pv, layer, q, qsb, qsh, pre, stream);
+        if (rc) return rc;
+    }
+    OwnParams own;
+    own.rows = rows; own.k = pv.plane(layer, 0, 0); own.v = pv.plane(layer, 1, 0); own.plane_bytes = pv.plane_bytes(); own.q = q;
+    own.ml = reinterpret_cast<float2*>(ws + pl.own_ml); own.acc = reinterpret_cast<float*>(ws + pl.own_acc);
+    own.q_stride_b = qsb; own.q_stride_h = qsh; own.splits = pl.splits; own.scale_log2 = sm_scale * kLog2e;
+    MergeParams mrg;
+    mrg.rows = rows; mrg.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); mrg.pre_acc = reinterpret_cast<float*>(ws + pl.pre_acc);
+    mrg.own_ml = own.ml; mrg.own_acc = own.acc; mrg.splits = pl.splits; mrg.ctas = prefix_ctas(); mrg.tiles = pl.tiles;
+    mrg.out = out; mrg.lse = lse; mrg.epi = epi;
     auto run = [&](auto part, auto merge) {
-        part<<<(unsigned)pl.parts, kPartWarps * 32, 0, stream>>>(prm);
+        part<<<B * pv.H * pl.splits, kPartWarps * 32, 0, stream>>>(own);
         if (cudaGetLastError() != cudaSuccess) return FPKV_ELAUNCH;
-        merge<<<B * Hq, pv.D, 0, stream>>>(prm);
+        merge<<<pl.tiles * pv.H * (kPrefixTileRows / 32) + (B * Hq + 31) / 32, 128, 0, stream>>>(mrg);
         return cudaGetLastError() == cudaSuccess ? FPKV_OK : FPKV_ELAUNCH;
     };
     if (pv.dtype == FPKV_BF16)
-        return pv.D == 128 ? run(shared_partial_kernel<__nv_bfloat16, 128>, shared_merge_kernel<__nv_bfloat16, 128>)
-                           : run(shared_partial_kernel<__nv_bfloat16, 64>, shared_merge_kernel<__nv_bfloat16, 64>);
-    return pv.D == 128 ? run(shared_partial_kernel<__half, 128>, shared_merge_kernel<__half, 128>)
-                       : run(shared_partial_kernel<__half, 64>, shared_merge_kernel<__half, 64>);
+        return pv.D == 128 ? run(own_part_kernel<__nv_bfloat16, 128>, shared_merge_kernel<__nv_bfloat16, 128>)
+                           : run(own_part_kernel<__nv_bfloat16, 64>, shared_merge_kernel<__nv_bfloat16, 64>);
+    return pv.D == 128 ? run(own_part_kernel<__half, 128>, shared_merge_kernel<__half, 128>)
+                       : run(own_part_kernel<__half, 64>, shared_merge_kernel<__half, 64>);
 }
 
 }  // namespace fpkv

@@ -1,0 +1,119 @@
+// What the two halves of shared-prefix decode attention agree on: rows, groups, and how the prefixes' key tiles are shared out.
+#pragma once
+
+#include "common.cuh"
+
+namespace fpkv {
+
+// The batch as the kernels see it.
+struct RowParams {
+    const int64_t* page_table;
+    const int64_t* p2l;
+    const int64_t* batch_idx;
+    const void* pos;
+    const int4* groups;                        // {first row, rows, shared pages, 0}
+    const int* row_group;
+    int32_t* status;
+    int B, Hq, H, n_rep, n_groups, n_pages, max_batch, pos_is_64;
+    int rows_per_tile;                         // batch rows of a query tile of the prefix part
+};
+
+struct PrefixParams {
+    RowParams rows;
+    float2* ml;                                // partials [slot][128 rows] (m, l): maximum and sum in base 2
+    float* acc;                                // [slot][D/4][128 rows][4]
+    int rows_per_plane, q_box_rows;
+    float scale_log2;
+};
+
+constexpr int kPrefixTileRows = 128;
+
+int prefix_ctas();
+bool prefix_supported(const PoolView& pv);
+int launch_prefix(const PoolView& pv, int layer, const void* q, long long q_stride_b, long long q_stride_h, PrefixParams prm, cudaStream_t stream);
+
+// Visible keys of a row and its slot; a slot or position out of range gives none.
+__device__ __forceinline__ int row_keys(const RowParams& p, int b, int* slot, bool report) {
+    const long long s = p.batch_idx[b];
+    const long long at = p.pos_is_64 ? reinterpret_cast<const int64_t*>(p.pos)[b] : (long long)reinterpret_cast<const int32_t*>(p.pos)[b];
+    *slot = 0;
+    if (s < 0 || s >= p.max_batch) { if (report) raise_status(p.status, FPKV_STATUS_BAD_SLOT); return 0; }
+    if (at < 0 || at / 128 >= p.n_pages) { if (report) raise_status(p.status, FPKV_STATUS_BAD_POS); return 0; }
+    *slot = (int)s;
+    return (int)at + 1;
+}
+// A group as the kernels use it: rows inside the batch and pages inside the table, or nothing.
+__device__ __forceinline__ int4 group_at(const RowParams& p, int g) {
+    int4 d = p.groups[g];
+    if (d.x < 0 || d.y <= 0 || d.x >= p.B || d.y > p.B - d.x || d.z <= 0) d.y = d.z = 0;
+    d.z = min(d.z, p.n_pages);
+    return d;
+}
+__device__ __forceinline__ int tiles_of(const RowParams& p, const int4& d) { return (d.y + p.rows_per_tile - 1) / p.rows_per_tile; }
+// Group of a row, -1 for none.
+__device__ __forceinline__ int group_of_row(const RowParams& p, int b, int4* d) {
+    const int g = p.n_groups > 0 ? p.row_group[b] : -1;
+    if (g < 0 || g >= p.n_groups) return -1;
+    *d = group_at(p, g);
+    return (d->y > 0 && b >= d->x && b < d->x + d->y) ? g : -1;
+}
+
+// ---- the schedule: key tiles of all segments in a row -- group by group, head by head, query tile by query tile -- in equal
+// shares.  flat_before[g], mt_before[g]: key tiles (over all segments) and query tiles before group g. --------------------
+// No share is empty: with fewer key tiles than CTAs, the first CTAs have one each.
+__device__ __forceinline__ int sharers(long long total, int ctas) { return (int)min((long long)ctas, total); }
+__device__ __forceinline__ long long share_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
+// The CTA whose share holds a position below the total.
+__device__ __forceinline__ int share_of(long long total, long long pos, int ctas) {
+    int c = (int)min(pos * ctas / total, (long long)(ctas - 1));
+    while (c + 1 < ctas && share_begin(total, c + 1, ctas) <= pos) ++c;
+    while (c > 0 && share_begin(total, c, ctas) > pos) --c;
+    return c;
+}
+__device__ __forceinline__ void prefix_schedule(const RowParams& p, long long* flat_before, int* mt_before, int lane) {      // one warp
+    long long flat = 0;
+    int mt = 0;
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        const int4 d = g < p.n_groups ? group_at(p, g) : make_int4(0, 0, 0, 0);
+        const int t = tiles_of(p, d);
+        long long f = (long long)t * p.H * d.z;
+        int m = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long yf = __shfl_up_sync(0xffffffffu, f, o);
+            const int ym = __shfl_up_sync(0xffffffffu, m, o);
+            if (lane >= o) { f += yf; m += ym; }
+        }
+        if (g < p.n_groups) { flat_before[g + 1] = flat + f; mt_before[g + 1] = mt + m; }
+        flat += __shfl_sync(0xffffffffu, f, 31);
+        mt += __shfl_sync(0xffffffffu, m, 31);
+    }
+    if (lane == 0) { flat_before[0] = 0; mt_before[0] = 0; }
+}
+struct Segment {
+    int index;                                 // over all groups
+    int b0, rows, h;                           // first batch row, query rows, stored head
+    int pages, tile;                           // key tiles of the segment; the one at the position asked for
+    int slot0;                                 // slot whose table names the pages
+};
+__device__ __forceinline__ Segment segment_at(const RowParams& p, const long long* flat_before, const int* mt_before, long long pos) {
+    int lo = 0, hi = p.n_groups;               // flat_before[lo] <= pos < flat_before[hi]
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (flat_before[mid] <= pos) lo = mid; else hi = mid; }
+    const int4 d = group_at(p, lo);
+    const int mt = mt_before[lo + 1] - mt_before[lo];
+    const long long rel = pos - flat_before[lo];
+    const int seg = (int)(rel / d.z), m = seg % mt;
+    Segment s;
+    s.tile = (int)(rel - (long long)seg * d.z);
+    s.pages = d.z;
+    s.h = seg / mt;
+    s.index = mt_before[lo] * p.H + seg;
+    s.b0 = d.x + m * p.rows_per_tile;
+    s.rows = min(p.rows_per_tile, d.x + d.y - s.b0) * p.n_rep;
+    const long long slot = p.batch_idx[d.x];
+    s.slot0 = slot >= 0 && slot < p.max_batch ? (int)slot : 0;
+    return s;
+}
+
+}  // namespace fpkv

@@ -566,7 +566,7 @@ class PagedKVCache(KVCacheBase):
         rows have in common are read once for all of them; the result is the same.
         Pools that ``fpkv_decode_attn_shared`` does not take (fp32, split layout,
         page sizes other than 128, more than 16 query heads per stored head) are
-        served row by row as without it."""
+        served row by row as without it, as is a scale that is not positive."""
         B, Hq, S, D = q.shape
         assert S == 1, "decode attention takes one query token per row"
         assert D == self.head_dim and Hq % self.n_heads == 0, "head layout must match the pool"
@@ -590,7 +590,7 @@ class PagedKVCache(KVCacheBase):
             lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=q.device)
         if shared is not None:
             assert shared.row_group.shape == (B,), "the prefix groups are those of another batch"
-            if shared.n_groups and self._shared_supported(Hq):
+            if shared.n_groups and B and self._shared_supported(Hq) and (sm_scale is None or sm_scale > 0):
                 self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared)
                 return out, lse
         ws = self._get_workspace(B, Hq)
@@ -653,6 +653,8 @@ class PagedKVCache(KVCacheBase):
 
     def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared):
         B, Hq, _, D = q.shape
+        if 0 in (q.stride(0), q.stride(1)):
+            q = q.contiguous()                      # the kernel's tensor map has no room for a repeated row
         assert shared.groups.is_cuda and shared.groups.is_contiguous() and shared.groups.dtype == torch.int32
         assert shared.row_group.is_cuda and shared.row_group.is_contiguous() and shared.row_group.dtype == torch.int32
         need = ctypes.c_size_t(0)

@@ -412,7 +412,9 @@ FPKV_API int fpkv_decode_attn_static(const fpkv_pool* pool, int32_t layer,
  * unmapped page are not visible, as in fpkv_decode_attn.
  * Takes 16-bit pools in the uniform layout with page_size 128, head_dim 64 or
  * 128 and at most 16 query heads per stored head (FPKV_ESHAPE / FPKV_EDTYPE
- * otherwise); n_groups <= FPKV_MAX_GROUPS.
+ * otherwise); n_groups <= FPKV_MAX_GROUPS, sm_scale > 0, q's strides not 0.
+ * A value row of the shared prefix that one row of a group sees must be finite
+ * also for those of its rows whose position lies before it.
  * workspace: device, 16-byte aligned, at least fpkv_decode_shared_workspace_bytes()
  * bytes, of any content; two calls that share one must not overlap.
  */

@@ -135,9 +135,9 @@ def test_shared_attention_validation():
     p, buf = _pool()
     ptr, need = buf.data_ptr(), ctypes.c_size_t(0)
 
-    def call(pool=p, out=ptr, q=ptr, sb=256, hq=4, B=2, pt=0, groups=ptr, n=1, rg=ptr, ws=ptr, size=1 << 40):
+    def call(pool=p, out=ptr, q=ptr, sb=256, hq=4, B=2, pt=0, groups=ptr, n=1, rg=ptr, ws=ptr, size=1 << 40, scale=0.125):
         return L.fpkv_decode_attn_shared(ctypes.byref(pool), 0, out, ptr, q, sb, 64, ptr, ptr, pt, B, hq, groups, n, rg,
-                                         0.125, ws, size, None, None, None)
+                                         scale, ws, size, None, None, None)
     assert call(_pool(dtype=_lib.FPKV_F32)[0]) == -7
     assert call(_pool(page_size=64)[0]) == -2 and call(_pool(split_q_heads=4)[0]) == -2
     assert call(_pool(head_dim=96)[0]) == -2
@@ -146,6 +146,7 @@ def test_shared_attention_validation():
     assert call(out=0) == -1 and call(q=0) == -1 and call(groups=0) == -1 and call(rg=0) == -1 and call(ws=0) == -1
     assert call(q=ptr + 2) == -3 and call(sb=100) == -3 and call(groups=ptr + 4) == -3 and call(rg=ptr + 2) == -3
     assert call(ws=ptr + 8) == -3 and call(size=64) == -6
+    assert call(scale=0.0) == -1 and call(scale=-1.0) == -1
     assert call(B=0) == 0
     assert L.fpkv_decode_shared_workspace_bytes(ctypes.byref(p), 2, 4, 1, ctypes.byref(need)) == 0 and need.value > 0
     assert L.fpkv_decode_shared_workspace_bytes(ctypes.byref(p), 2, 4, 1, None) == -1
