@@ -111,6 +111,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;");     // the own part needs nothing from here
     const uint32_t tmem = (uint32_t)*tmem_slot;
     // S/P of side 0 [0,128), of side 1 [128,256), O of side 0 [256,384), of side 1 [384,512)
     bool alive = true;
