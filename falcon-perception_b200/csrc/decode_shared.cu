@@ -7,48 +7,56 @@
 // once a group instead of once a row.  Three launches:
 //
 //  * prefix part: shared_prefix_tc.cu.
-//  * own part, below: a CTA takes up to 8 query heads of one stored head of one batch row and a share of the row's keys
-//    behind the prefix.  Its warps walk blocks of 16 keys with mma.sync.m16n8k16,
-//        S^T = K Q^T   (16 keys x 8 heads),   O^T += V^T P^T   (dims x 8 heads)
-//    and K and V go from memory straight into the registers of the MMAs: the order of the contraction index and of the
-//    output's dims is free, so it is chosen such that every lane's 16-byte piece of a row is its own operand.  No shared
-//    memory and no barrier in the loop; 16 warps an SM keep 128 KB of loads in flight.  Bound by the bytes of the rows' own
-//    keys.
+//  * own part, below: the rows' own keys in blocks of 16, for every row and every 8 query heads of a stored head, one after
+//    the other, in equal shares, one per WARP: a warp needs no other, so there is no barrier, and all have the same to do
+//    however the lengths differ.  A block is
+//        S^T = K Q^T   (16 keys x 8 heads),   O^T += V^T P^T   (dims x 8 heads)      in mma.sync.m16n8k16,
+//    K and V come by tensor copies (16 rows, 128-byte swizzle) into a ring of the warp's own, requested several blocks ahead
+//    and across rows: with only what fits the registers in flight, 12 warps an SM reached 3.7 TB/s.  The order of the
+//    contraction index and of the output's dims is free, so it is chosen such that every lane's 16-byte piece of a row is its
+//    own operand and no access to the ring conflicts.  Bound by the bytes of the rows' own keys.
 //  * merge: joins the partials of every (row, head), applies the sink gate, writes out and lse.
 // The three are chained by programmatic dependent launch: the own part starts as soon as every CTA of the prefix part has
 // (it needs nothing from it) and fills the SMs as they come free; it ends after the prefix part, so that the merge, whose
 // set-up overlaps both, has only the own part to wait for.
 
+#include "tc5.cuh"
 #include "shared_prefix.cuh"
 
 namespace fpkv {
 
 namespace {
 
-constexpr int kPage = 128;
 constexpr int kMaxRep = 16;                    // query heads of a stored head
 constexpr int kHeads = 8;                      // of them, those of a CTA of the own part: the MMAs' columns
-constexpr int kPartWarps = 4;
-constexpr int kListTiles = 64;                 // pages resolved at a time
+// One CTA an SM.  A block takes a warp about 1200 clocks from its arrival (products, maximum, exponentials, products, each
+// waiting for the one before), so it takes many warps to keep up with memory: 12 with two blocks of 16 keys each did 256 rows
+// of 1 to 512 own keys faster than 8 with three.
+constexpr int kOwnWarps = 12;
+constexpr int kRingBytes = 16 * 1024;          // of a warp
+constexpr int kBlock = 16, kPageBlocks = kPage / kBlock;
+constexpr int kMaxRows = 1024;                 // batch rows of a launch of the own part
 
 struct OwnParams {
     RowParams rows;
-    const char* k;                             // K plane of stored head 0
-    const char* v;
-    size_t plane_bytes;
     const void* q;
-    float2* ml;                                // partials [B][Hq][splits] (m, l)
-    float* acc;                                // [B][Hq][splits][D]
+    // partials [slot][8 heads] (m, l) and [slot][8 heads][D]; slot = worker number + segment number, segments counted row by
+    // row, stored head by stored head, 8 query heads by 8 query heads
+    float2* ml;
+    float* acc;
+    long long* before;                         // [rows + 1] blocks of all segments before a row, for the merge
     long long q_stride_b, q_stride_h;
-    int splits, head_blocks;                   // shares of a row's keys; blocks of kHeads query heads of a stored head
+    int row0, n_rows, head_blocks;             // the launch's rows; blocks of kHeads query heads of a stored head
+    int rows_per_plane;
     float scale_log2;
 };
 
 struct MergeParams {
     RowParams rows;
     const float2* pre_ml; const float* pre_acc;
-    const float2* own_ml; const float* own_acc;
-    int splits, ctas, tiles;                   // of the own part; of the prefix part; upper bound of its query tiles
+    const float2* own_ml; const float* own_acc; const long long* own_before;
+    size_t own_slots;                          // partials of one launch of the own part
+    int workers, head_blocks, ctas, tiles;     // of the own part; of the prefix part, upper bound of its query tiles
     void* out;
     float* lse;
     Epilogue epi;
@@ -81,167 +89,273 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     return y;
 }
 
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kPartWarps * 32, 4)
-own_part_kernel(const OwnParams prm)
+__global__ void __launch_bounds__(kOwnWarps * 32, 1)
+own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
 {
-    constexpr int NI = D / 32, NH = D / 64;    // 16-byte pieces of a K row per lane; 64-column groups of a V row
+    constexpr int NH = D / 64;                 // 64-column groups of a row
+    constexpr int kHalf = kBlock * 128, kTile = NH * kHalf;  // a block's K (or V): column groups of 16 rows of 128 bytes
+    constexpr int kStages = kRingBytes / (2 * kTile);
     const RowParams& rp = prm.rows;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
-    __shared__ int s_row[kListTiles];          // pool row of each resolved page, -1 = not visible
-    __shared__ float s_m[kPartWarps][kHeads], s_l[kPartWarps][kHeads];
-    __shared__ __align__(16) float s_acc[kPartWarps][kHeads][D + 4];
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ long long s_before[kMaxRows + 1];
+    __shared__ int s_slot[kMaxRows], s_first[kMaxRows], s_keys[kMaxRows];    // slot, first own page, visible keys of each row
+    __shared__ uint64_t s_bars[kOwnWarps][kStages];
+    __shared__ int s_abort;
     asm volatile("griddepcontrol.launch_dependents;");       // the merge may take its seats
+    const uint32_t ring = ((s32(smem_raw) + 1023u) & ~1023u) + warp * kRingBytes, bars = s32(&s_bars[warp][0]);
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
+        s_abort = 0;
+    }
+    if (lane < kStages) bar_init(bars + 8 * lane, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 
-    int id = blockIdx.x;
-    const int split = id % prm.splits; id /= prm.splits;
-    const int r0 = (id % prm.head_blocks) * kHeads; id /= prm.head_blocks;
-    const int h = id % rp.H, b0 = id / rp.H;
-    const int heads = min(kHeads, rp.n_rep - r0);
-    int slot0; int4 d;
-    const int keys = row_keys(rp, b0, &slot0, h == 0 && split == 0 && r0 == 0 && threadIdx.x == 0);
-    const int first_page = group_of_row(rp, b0, &d) >= 0 ? d.z : 0, end_page = (keys + kPage - 1) / kPage;
-    const int n_pg = max(0, end_page - first_page);
-    const int pg0 = first_page + (int)((long long)n_pg * split / prm.splits), pg1 = first_page + (int)((long long)n_pg * (split + 1) / prm.splits);
-
-    // queries: head g, dims i * 32 + c * 8 .. + 7
-    uint4 qa[NI];
-    const T* q = reinterpret_cast<const T*>(prm.q) + b0 * prm.q_stride_b + (h * rp.n_rep + r0 + g) * prm.q_stride_h;
+    // ---- the schedule -----------------------------------------------------------------
+    const int n_segs = rp.H * prm.head_blocks;               // of a row
+    for (int i = threadIdx.x; i < prm.n_rows; i += kOwnWarps * 32) {
+        const int b = prm.row0 + i;
+        int slot; int4 d;
+        const int keys = row_keys(rp, b, &slot, blockIdx.x == 0);
+        const int first = group_of_row(rp, b, &d) >= 0 ? d.z : 0;
+        s_slot[i] = slot; s_first[i] = first; s_keys[i] = keys;
+        s_before[i + 1] = (long long)max(0, (keys + kBlock - 1) / kBlock - first * kPageBlocks) * n_segs;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        long long carry = 0;
+        for (int i0 = 0; i0 < prm.n_rows; i0 += 32) {
+            const int i = i0 + lane;
+            long long v = i < prm.n_rows ? s_before[i + 1] : 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) qa[i] = g < heads ? ld16(reinterpret_cast<const char*>(q + i * 32 + c * 8)) : make_uint4(0, 0, 0, 0);
-    float acc[NH][4][4];                       // O^T: rows dims a * 64 + g * 8 + 2 e (+ 1), columns heads 2 c and 2 c + 1
-#pragma unroll
-    for (int a = 0; a < NH; ++a)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[a][e][k] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2 c and 2 c + 1; l this lane's keys alone
-    const char* kp = prm.k + (size_t)h * prm.plane_bytes;
-    const char* vp = prm.v + (size_t)h * prm.plane_bytes;
-
-    for (int p0 = pg0; p0 < pg1; p0 += kListTiles) {
-        __syncthreads();
-        for (int j = threadIdx.x; j < min(kListTiles, pg1 - p0); j += kPartWarps * 32) {
-            const long long pg = rp.page_table[(long long)slot0 * rp.n_pages + p0 + j];
-            int row = -1;
-            if (pg >= rp.n_pages) raise_status(rp.status, FPKV_STATUS_BAD_PAGE);
-            else if (pg >= 0 && rp.p2l[(long long)slot0 * rp.n_pages + pg] >= 0) row = (int)pg * kPage;
-            s_row[j] = row;
+            for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += y; }
+            if (i < prm.n_rows) s_before[i + 1] = v + carry;
+            carry += __shfl_sync(0xffffffffu, v, 31);
         }
-        __syncthreads();
-        const int blocks = min(kListTiles, pg1 - p0) * (kPage / 16);
-        for (int k16 = warp; k16 < blocks; k16 += kPartWarps) {
-            const int row0 = s_row[k16 / (kPage / 16)];
-            const int key0 = p0 * kPage + k16 * 16;
-            if (row0 < 0 || key0 >= keys) continue;
-            const size_t at = (size_t)(row0 + (k16 % (kPage / 16)) * 16);
-            uint4 kk[2][NI], vv[4][NH];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)        // keys g and g + 8 of the block
-#pragma unroll
-                for (int i = 0; i < NI; ++i) kk[j][i] = ld16(kp + ((at + j * 8 + g) * D + i * 32 + c * 8) * 2);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)        // keys 2c, 2c + 1, 2c + 8, 2c + 9
-#pragma unroll
-                for (int a = 0; a < NH; ++a) vv[k][a] = ld16(vp + ((at + 2 * c + (k & 1) + (k >> 1) * 8) * D + a * 64 + g * 8) * 2);
-            float s[4] = {0.f, 0.f, 0.f, 0.f}; // S^T: keys g (0, 1) and g + 8 (2, 3), heads 2 c and 2 c + 1
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const uint32_t a0[4] = {kk[0][i].x, kk[1][i].x, kk[0][i].y, kk[1][i].y}, a1[4] = {kk[0][i].z, kk[1][i].z, kk[0][i].w, kk[1][i].w};
-                mma16816<T>(s, a0, qa[i].x, qa[i].y);
-                mma16816<T>(s, a1, qa[i].z, qa[i].w);
+        if (lane == 0) s_before[0] = 0;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) for (int i = threadIdx.x; i <= prm.n_rows; i += kOwnWarps * 32) prm.before[i] = s_before[i];
+    const long long total = s_before[prm.n_rows];
+    const int workers = sharers(total, gridDim.x * kOwnWarps), me = blockIdx.x * kOwnWarps + warp;
+    long long pos = me < workers ? share_begin(total, me, workers) : 0;
+    const long long end = me < workers ? share_begin(total, me + 1, workers) : 0;
+
+    // A piece: blocks [blk0, blk0 + n) of a segment.
+    struct Piece { int row, first, keys, seg, blk0, n, h; };
+    auto piece_at = [&](long long at) -> Piece {
+        int lo = 0, hi = prm.n_rows;                         // s_before[lo] <= at < s_before[hi]
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_before[mid] <= at) lo = mid; else hi = mid; }
+        Piece p;
+        p.row = lo; p.first = s_first[lo]; p.keys = s_keys[lo];
+        const int nb = (p.keys + kBlock - 1) / kBlock - p.first * kPageBlocks;
+        const unsigned rel = (unsigned)(at - s_before[lo]);  // blocks of one row
+        p.seg = (int)(rel / (unsigned)nb); p.blk0 = (int)(rel - (unsigned)p.seg * nb);
+        p.n = (int)min((long long)(nb - p.blk0), end - at);
+        p.h = p.seg / prm.head_blocks;
+        return p;
+    };
+    // ---- requests run ahead of the work, across pieces -------------------------------------
+    // Pages of a piece are looked up 32 at a time, one a lane; the table entries of the first 32 of the piece after next are on
+    // their way while the present one is requested.
+    auto page_of = [&](const Piece& p, int w) -> long long {
+        const int page = p.first + p.blk0 / kPageBlocks + w * 32 + lane;
+        return page * kPage < p.keys ? rp.page_table[(long long)s_slot[p.row] * rp.n_pages + page] : -1;
+    };
+    Piece ahead, next;                                       // the piece that is being requested, the one after it
+    long long next_pos = pos, next_page = -1;                // end of `next`; this lane's table entry of it
+    auto advance = [&]() {
+        if (next_pos >= end) { next.n = 0; return; }
+        next = piece_at(next_pos);
+        next_pos += next.n;
+        next_page = page_of(next, 0);
+    };
+    advance();
+    int ahead_t = 0, window = 0, pool_rows = -1;             // pool rows of 32 pages of `ahead`; -1 = not visible
+    ahead.n = 0;
+    uint32_t requested = 0, visible = 0;                     // blocks requested; of the stages' blocks, those on visible pages
+    auto request = [&]() {
+        bool lookup = false;
+        long long pg = -1;
+        if (ahead_t == ahead.n) {
+            if (next.n == 0) return;
+            ahead = next; pg = next_page; ahead_t = 0; window = 0;
+            lookup = true;
+            advance();
+            // the queries will be wanted soon
+            if (lane < min(kHeads, rp.n_rep) * NH) {
+                const int r0 = (ahead.seg % prm.head_blocks) * kHeads + lane / NH;
+                if (r0 < rp.n_rep)
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T*>(prm.q) + (prm.row0 + ahead.row) * prm.q_stride_b +
+                                                                   (ahead.h * rp.n_rep + r0) * prm.q_stride_h + lane % NH * 64));
             }
-            // keys past the row's end: no weight, and (never appended, perhaps) no value either
-            float mx[2];
-            if (key0 + 16 > keys) {
+        }
+        const int at_blk = ahead.blk0 + ahead_t, p = at_blk / kPageBlocks, w = (p - ahead.blk0 / kPageBlocks) / 32;
+        if (w != window) { window = w; pg = page_of(ahead, w); lookup = true; }
+        if (lookup) {
+            pool_rows = -1;
+            if (pg >= rp.n_pages) raise_status(rp.status, FPKV_STATUS_BAD_PAGE);
+            else if (pg >= 0 && rp.p2l[(long long)s_slot[ahead.row] * rp.n_pages + pg] >= 0) pool_rows = (int)pg * kPage;
+        }
+        const int row0 = __shfl_sync(0xffffffffu, pool_rows, (p - ahead.blk0 / kPageBlocks) % 32);
+        const uint32_t st = requested % kStages;
+        visible = row0 >= 0 ? visible | (1u << st) : visible & ~(1u << st);
+        if (lane == 0) {
+            const uint32_t bar = bars + 8 * st, dst = ring + st * (2 * kTile);
+            if (row0 >= 0) {
+                const int row = ahead.h * prm.rows_per_plane + row0 + at_blk % kPageBlocks * kBlock;
+                bar_expect_tx(bar, 2 * kTile);
+                tma_3d(dst, &map, 0, row, 0, bar);
+                tma_3d(dst + kTile, &map, 0, row + rp.H * prm.rows_per_plane, 0, bar);
+            } else bar_arrive(bar);
+        }
+        ++requested; ++ahead_t;
+    };
+    const uint32_t n_blocks = (uint32_t)(end - pos);
+    for (int i = 0; i < kStages; ++i) request();
+    uint32_t done = 0;
+    bool alive = true;
+    while (pos < end && alive) {
+        const Piece pc = piece_at(pos);
+        pos += pc.n;
+        const int r0 = (pc.seg % prm.head_blocks) * kHeads, heads = min(kHeads, rp.n_rep - r0);
+        // queries: head g, dims a * 64 + c * 16 + e * 8 .. + 7
+        uint4 qa[NH][2];
+        const T* q = reinterpret_cast<const T*>(prm.q) + (prm.row0 + pc.row) * prm.q_stride_b + (pc.h * rp.n_rep + r0 + g) * prm.q_stride_h;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) if (key0 + g + (e >> 1) * 8 >= keys) s[e] = -INFINITY;
+        for (int a = 0; a < NH; ++a)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qa[a][e] = g < heads ? ld16(reinterpret_cast<const char*>(q + a * 64 + c * 16 + e * 8)) : make_uint4(0, 0, 0, 0);
+        float acc[NH][4][4];                   // O^T: rows dims a * 64 + g * 8 + 2 e (+ 1), columns heads 2 c and 2 c + 1
+#pragma unroll
+        for (int a = 0; a < NH; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[a][e][k] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // heads 2 c and 2 c + 1; l this lane's keys alone
+
+        for (int t = 0; t < pc.n; ++t, ++done) {
+            const uint32_t st = done % kStages;
+            if (!bar_wait(bars + 8 * st, (done / kStages) & 1u, &s_abort)) { alive = false; break; }
+            if (visible >> st & 1u) {
+                const int key0 = pc.first * kPage + (pc.blk0 + t) * kBlock;
+                const uint32_t ks = ring + st * (2 * kTile), vs = ks + kTile;
+                // keys g and g + 8: 16-byte pieces 2 c and 2 c + 1 of their rows (row & 7 = g); two chains of products
+                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int a = 0; a < NH; ++a)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t at = ks + a * kHalf + g * 128 + (((2 * c + e) ^ g) << 4);
+                        const uint4 k0 = lds16(at), k1 = lds16(at + 8 * 128);
+                        const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+                        mma16816<T>(s, a0, qa[a][e].x, qa[a][e].y);
+                        mma16816<T>(s2, a1, qa[a][e].z, qa[a][e].w);
+                    }
+                uint4 v[4][NH];                // keys 2c, 2c + 1, 2c + 8, 2c + 9: piece g
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (key0 + 2 * c + (k & 1) + (k >> 1) * 8 >= keys)
 #pragma unroll
-                        for (int a = 0; a < NH; ++a) vv[k][a] = make_uint4(0, 0, 0, 0);
-            }
+                    for (int a = 0; a < NH; ++a) {
+                        const int r = 2 * c + (k & 1) + (k >> 1) * 8;
+                        v[k][a] = lds16(vs + a * kHalf + r * 128 + ((g ^ (r & 7)) << 4));
+                    }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                mx[r] = fmaxf(s[r], s[2 + r]);                             // the scale is positive: the maximum commutes with it
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 4));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 8));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 16)) * prm.scale_log2;
-            }
-            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+                for (int e = 0; e < 4; ++e) s[e] += s2[e];   // S^T: keys g (0, 1) and g + 8 (2, 3), heads 2 c and 2 c + 1
+                // keys past the row's end: no weight, and (never appended, perhaps) no value either
+                if (key0 + kBlock > pc.keys) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (key0 + g + (e >> 1) * 8 >= pc.keys) s[e] = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (key0 + 2 * c + (k & 1) + (k >> 1) * 8 >= pc.keys)
+#pragma unroll
+                            for (int a = 0; a < NH; ++a) v[k][a] = make_uint4(0, 0, 0, 0);
+                }
+                float mx[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float mn = fmaxf(m[r], mx[r]), alpha = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn);
-                    m[r] = mn;
-                    l[r] *= alpha;
-#pragma unroll
-                    for (int a = 0; a < NH; ++a)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { acc[a][e][r] *= alpha; acc[a][e][2 + r] *= alpha; }
+                    mx[r] = fmaxf(s[r], s[2 + r]);           // the scale is positive: the maximum commutes with it
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 4));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 8));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 16)) * prm.scale_log2;
                 }
-            }
+                if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = e & 1;
-                s[e] = m[r] == -INFINITY ? 0.f : exp2f(s[e] * prm.scale_log2 - m[r]);
-                l[r] += s[e];
-            }
-            const uint32_t b0_ = transposed(pack_pair<T>(s[0], s[1])), b1_ = transposed(pack_pair<T>(s[2], s[3]));
+                    for (int r = 0; r < 2; ++r) {
+                        const float mn = fmaxf(m[r], mx[r]), alpha = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn);
+                        m[r] = mn;
+                        l[r] *= alpha;
 #pragma unroll
-            for (int a = 0; a < NH; ++a) {
-                const uint32_t* x0 = &vv[0][a].x; const uint32_t* x1 = &vv[1][a].x;
-                const uint32_t* x2 = &vv[2][a].x; const uint32_t* x3 = &vv[3][a].x;
+                        for (int a = 0; a < NH; ++a)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { acc[a][e][r] *= alpha; acc[a][e][2 + r] *= alpha; }
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t at_[4] = {__byte_perm(x0[e], x1[e], 0x5410u), __byte_perm(x0[e], x1[e], 0x7632u),
-                                             __byte_perm(x2[e], x3[e], 0x5410u), __byte_perm(x2[e], x3[e], 0x7632u)};
-                    mma16816<T>(acc[a][e], at_, b0_, b1_);
+                    const int r = e & 1;
+                    s[e] = m[r] == -INFINITY ? 0.f : exp2f(s[e] * prm.scale_log2 - m[r]);
+                    l[r] += s[e];
+                }
+                const uint32_t p0 = transposed(pack_pair<T>(s[0], s[1])), p1 = transposed(pack_pair<T>(s[2], s[3]));
+#pragma unroll
+                for (int a = 0; a < NH; ++a) {
+                    const uint32_t* x0 = &v[0][a].x; const uint32_t* x1 = &v[1][a].x;
+                    const uint32_t* x2 = &v[2][a].x; const uint32_t* x3 = &v[3][a].x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t vt[4] = {__byte_perm(x0[e], x1[e], 0x5410u), __byte_perm(x0[e], x1[e], 0x7632u),
+                                                __byte_perm(x2[e], x3[e], 0x5410u), __byte_perm(x2[e], x3[e], 0x7632u)};
+                        mma16816<T>(acc[a][e], vt, p0, p1);
+                    }
                 }
             }
+            __syncwarp();                      // all lanes have read the stage
+            if (requested < n_blocks) request();
+        }
+        if (!alive) break;
+        // ---- the piece's partial --------------------------------------------------------
+        const size_t slot = (size_t)me + (size_t)pc.row * n_segs + pc.seg;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+            const int head = 2 * c + r;
+            if (head >= heads) continue;
+            if (g == 0) prm.ml[slot * kHeads + head] = make_float2(m[r], l[r]);
+            float4* dst = reinterpret_cast<float4*>(prm.acc + (slot * kHeads + head) * D + g * 8);
+#pragma unroll
+            for (int a = 0; a < NH; ++a)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    dst[a * 16 + e] = make_float4(acc[a][2 * e][r], acc[a][2 * e][2 + r], acc[a][2 * e + 1][r], acc[a][2 * e + 1][2 + r]);
         }
     }
-    // ---- join the warps, write the partial ------------------------------------------
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-        if (g == 0) { s_m[warp][2 * c + r] = m[r]; s_l[warp][2 * c + r] = l[r]; }
-    }
-#pragma unroll
-    for (int a = 0; a < NH; ++a)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s_acc[warp][2 * c + (k & 1)][a * 64 + g * 8 + 2 * e + (k >> 1)] = acc[a][e][k];
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * (D / 4); i += kPartWarps * 32) {
-        const int r = i / (D / 4), col = i % (D / 4) * 4;
-        const size_t part = ((size_t)b0 * rp.Hq + h * rp.n_rep + r0 + r) * prm.splits + split;
-        float M = -INFINITY;
-        for (int w = 0; w < kPartWarps; ++w) M = fmaxf(M, s_m[w][r]);
-        float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < kPartWarps; ++w) {
-            if (s_m[w][r] == -INFINITY) continue;
-            const float f = exp2f(s_m[w][r] - M);
-            const float4 v = *reinterpret_cast<const float4*>(&s_acc[w][r][col]);
-            L += s_l[w][r] * f;
-            o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
-        }
-        *reinterpret_cast<float4*>(prm.acc + part * D + col) = make_float4(o[0], o[1], o[2], o[3]);
-        if (col == 0) prm.ml[part] = make_float2(M, L);
+    if (!alive) {                              // a copy did not come: say so, and wait (bounded) for those in flight
+        if (lane == 0) { raise_status(rp.status, FPKV_STATUS_TIMEOUT); *reinterpret_cast<volatile int*>(&s_abort) = 1; }
+        for (; done < requested; ++done)
+            for (uint32_t k = 0; k < kSpin && !bar_try(bars + 8 * (done % kStages), (done / kStages) & 1u); ++k) {}
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");       // not done before the prefix part is
 }
 
-// Block: 32 (row, head) pairs, one a lane, and 32 columns, eight a warp.  The pairs are a quarter of a query tile of the
-// prefix part, whose partials lie side by side; behind those blocks come some for the rows that are in no group.  The
-// weights of all partials are worked out first, in parallel, so that the loads of the sums do not wait for one another.
+// Block: 32 (row, head) pairs, one a lane, and 32 columns: four column groups x two halves of the partials, a warp each.  The
+// pairs are a quarter of a query tile of the prefix part, whose partials lie side by side; behind those blocks come some for
+// the rows that are in no group.  The weights of all partials are worked out first, in parallel, so that the loads of the sums
+// do not wait for one another.
 constexpr int kMergePieces = 32;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 shared_merge_kernel(const MergeParams prm)
 {
     constexpr int kColBlocks = D / 32;
@@ -249,8 +363,9 @@ shared_merge_kernel(const MergeParams prm)
     __shared__ long long flat_before[FPKV_MAX_GROUPS + 1];
     __shared__ int mt_before[FPKV_MAX_GROUPS + 1];
     __shared__ float2 s_ml[kMergePieces][32];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int col4 = (blockIdx.x % kColBlocks) * 8 + warp * 2, block = blockIdx.x / kColBlocks;
+    __shared__ float s_half[4][9][32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = warp / 4;
+    const int col4 = (blockIdx.x % kColBlocks) * 8 + warp % 4 * 2, block = blockIdx.x / kColBlocks;
     const int tile_blocks = prm.tiles * rp.H * (kPrefixTileRows / 32);
     int b = -1, hq = 0, c0 = 0, n_pre = 0, index = 0, trow = 0;
     if (block < tile_blocks) {
@@ -280,19 +395,37 @@ shared_merge_kernel(const MergeParams prm)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (__ballot_sync(0xffffffffu, b >= 0) == 0) return;     // the same for all warps
-    const size_t row = (size_t)max(b, 0) * rp.Hq + hq, own = row * prm.splits;
-    const int n = n_pre + prm.splits;
+    // the row's partials of the own part: first slot (times 8, plus the head) and number
+    size_t own = 0;
+    int n_own = 0;
+    if (b >= 0) {
+        const int chunk = b / kMaxRows, i = b % kMaxRows, rows = min(kMaxRows, rp.B - chunk * kMaxRows);
+        const long long* before = prm.own_before + (size_t)chunk * (kMaxRows + 1);
+        const long long at = before[i], blocks = before[i + 1] - at, total = before[rows];
+        if (blocks > 0) {
+            const int n_segs = rp.H * prm.head_blocks, rep = hq % rp.n_rep, seg = hq / rp.n_rep * prm.head_blocks + rep / kHeads;
+            const long long nb = blocks / n_segs, first = at + nb * seg;
+            const int workers = sharers(total, prm.workers), w0 = share_of(total, first, workers);
+            n_own = share_of(total, first + nb - 1, workers) - w0 + 1;
+            own = ((size_t)chunk * prm.own_slots + (size_t)w0 + (size_t)i * n_segs + seg) * kHeads + rep % kHeads;
+        }
+    }
+    const int n = n_pre + (int)__reduce_max_sync(0xffffffffu, (uint32_t)n_own);
     float M = -INFINITY, L = 0.f, a[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = 0.f;
     for (int p0 = 0; p0 < n; p0 += kMergePieces) {
         const int here = min(kMergePieces, n - p0);
         __syncthreads();
-#pragma unroll 8
-        for (int p = warp; p < here; p += 4) {
-            const int i = p0 + p;
-            s_ml[p][lane] = b < 0 ? make_float2(-INFINITY, 0.f)
-                                  : i < n_pre ? prm.pre_ml[(size_t)(c0 + i + index) * kPrefixTileRows + trow] : prm.own_ml[own + i - n_pre];
+#pragma unroll
+        for (int r = 0; r < kMergePieces / 8; ++r) {
+            const int p = warp + 8 * r, i = p0 + p;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (p < here && b >= 0) {
+                if (i < n_pre) ml = prm.pre_ml[(size_t)(c0 + i + index) * kPrefixTileRows + trow];
+                else if (i - n_pre < n_own) ml = prm.own_ml[own + (size_t)(i - n_pre) * kHeads];
+            }
+            s_ml[p][lane] = ml;
         }
         __syncthreads();
         float mn = M;
@@ -303,11 +436,11 @@ shared_merge_kernel(const MergeParams prm)
 #pragma unroll
         for (int k = 0; k < 8; ++k) a[k] *= alpha;
 #pragma unroll 8
-        for (int p = 0; p < here; ++p) {
+        for (int p = half; p < here; p += 2) {
             const float2 ml = s_ml[p][lane];
             const int i = p0 + p;
             const float4* src = i < n_pre ? reinterpret_cast<const float4*>(prm.pre_acc) + ((size_t)(c0 + i + index) * (D / 4) + col4) * kPrefixTileRows + trow
-                                          : reinterpret_cast<const float4*>(prm.own_acc) + (own + i - n_pre) * (D / 4) + col4;
+                                          : reinterpret_cast<const float4*>(prm.own_acc) + (own + (size_t)(i - n_pre) * kHeads) * (D / 4) + col4;
             const size_t step = i < n_pre ? kPrefixTileRows : 1;
             const bool some = ml.y != 0.f;                   // nothing visible: no sums were written
             const float4 x = some ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f), y = some ? src[step] : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -317,7 +450,17 @@ shared_merge_kernel(const MergeParams prm)
             a[4] += w * y.x; a[5] += w * y.y; a[6] += w * y.z; a[7] += w * y.w;
         }
     }
-    if (b < 0) return;
+    if (half == 1) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s_half[warp - 4][k][lane] = a[k];
+        s_half[warp - 4][8][lane] = L;
+    }
+    __syncthreads();
+    if (half == 1 || b < 0) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] += s_half[warp][k][lane];
+    L += s_half[warp][8][lane];
+    const size_t row = (size_t)b * rp.Hq + hq;
     const float lse = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
     const float gate = sink_gate(prm.epi, hq, lse), inv = L == 0.f ? 0.f : 1.f / L;
     __align__(16) T o[8];
@@ -327,7 +470,7 @@ shared_merge_kernel(const MergeParams prm)
     if (col4 == 0) prm.lse[row] = lse;
 }
 
-struct Plan { int n_rep, rows_per_tile, tiles, splits, head_blocks; size_t slots, pre_ml, pre_acc, own_ml, own_acc, bytes; };
+struct Plan { int n_rep, rows_per_tile, tiles, head_blocks, workers, chunks; size_t slots, own_slots, pre_ml, pre_acc, own_ml, own_acc, own_before, bytes; };
 Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
 {
     Plan p;
@@ -336,15 +479,17 @@ Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
     // a group leaves at most one tile that is not full
     p.tiles = n_groups > 0 ? B / p.rows_per_tile + (n_groups < B ? n_groups : B) : 0;
     p.head_blocks = (p.n_rep + kHeads - 1) / kHeads;
-    // Own part: four CTAs an SM when there are few rows.
-    p.splits = 4 * 148 / (B * pv.H > 0 ? B * pv.H * p.head_blocks : 1);
-    p.splits = p.splits < 1 ? 1 : p.splits > 32 ? 32 : p.splits;
+    p.workers = prefix_ctas() * kOwnWarps;
+    p.chunks = (B + kMaxRows - 1) / kMaxRows;
+    // slots are worker (or CTA) number + segment number
     p.slots = p.tiles > 0 ? (size_t)p.tiles * pv.H + prefix_ctas() : 0;
+    p.own_slots = (size_t)(B < kMaxRows ? B : kMaxRows) * pv.H * p.head_blocks + p.workers;
     auto place = [at = (size_t)0](size_t n) mutable { const size_t was = at; at += (n + 255) / 256 * 256; return was; };
     p.pre_ml = place(p.slots * kPrefixTileRows * sizeof(float2));
     p.pre_acc = place(p.slots * kPrefixTileRows * pv.D * sizeof(float));
-    p.own_ml = place((size_t)B * Hq * p.splits * sizeof(float2));
-    p.own_acc = place((size_t)B * Hq * p.splits * pv.D * sizeof(float));
+    p.own_ml = place(p.chunks * p.own_slots * kHeads * sizeof(float2));
+    p.own_acc = place(p.chunks * p.own_slots * kHeads * pv.D * sizeof(float));
+    p.own_before = place((size_t)p.chunks * (kMaxRows + 1) * sizeof(long long));
     p.bytes = place(0);
     return p;
 }
@@ -378,26 +523,38 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
         if (rc) return rc;
     }
     OwnParams own;
-    own.rows = rows; own.k = pv.plane(layer, 0, 0); own.v = pv.plane(layer, 1, 0); own.plane_bytes = pv.plane_bytes(); own.q = q;
-    own.ml = reinterpret_cast<float2*>(ws + pl.own_ml); own.acc = reinterpret_cast<float*>(ws + pl.own_acc);
-    own.q_stride_b = qsb; own.q_stride_h = qsh; own.splits = pl.splits; own.head_blocks = pl.head_blocks; own.scale_log2 = sm_scale * kLog2e;
+    own.rows = rows; own.q = q; own.rows_per_plane = pv.n_pages * pv.P;
+    own.q_stride_b = qsb; own.q_stride_h = qsh; own.head_blocks = pl.head_blocks; own.scale_log2 = sm_scale * kLog2e;
     MergeParams mrg;
     mrg.rows = rows; mrg.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); mrg.pre_acc = reinterpret_cast<float*>(ws + pl.pre_acc);
-    mrg.own_ml = own.ml; mrg.own_acc = own.acc; mrg.splits = pl.splits; mrg.ctas = prefix_ctas(); mrg.tiles = pl.tiles;
+    mrg.own_ml = reinterpret_cast<float2*>(ws + pl.own_ml); mrg.own_acc = reinterpret_cast<float*>(ws + pl.own_acc);
+    mrg.own_before = reinterpret_cast<long long*>(ws + pl.own_before); mrg.own_slots = pl.own_slots;
+    mrg.workers = pl.workers; mrg.head_blocks = pl.head_blocks; mrg.ctas = prefix_ctas(); mrg.tiles = pl.tiles;
     mrg.out = out; mrg.lse = lse; mrg.epi = epi;
-    auto launch = [&](auto kern, int grid, bool chained, const auto& args) {
+    CUtensorMap map;
+    if (!encode_rows(&map, pv, layer, kBlock)) return FPKV_ELAUNCH;
+    constexpr int kOwnSmem = 1024 + kOwnWarps * kRingBytes;
+    auto launch = [&](auto kern, int grid, int threads, int smem, bool chained, const auto&... args) {
+        if (smem > 0 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(128); cfg.stream = stream;
+        cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr.val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = &attr; cfg.numAttrs = chained ? 1 : 0;
-        return cudaLaunchKernelEx(&cfg, kern, args) == cudaSuccess;
+        return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
     };
-    static_assert(kPartWarps * 32 == 128, "both kernels run blocks of 128 threads");
     auto run = [&](auto part, auto merge) {
+        // (launches of further rows wait for the one before: each ends after the prefix part, and so after all of its own kind)
+        for (int k = 0; k < pl.chunks; ++k) {
+            own.row0 = k * kMaxRows; own.n_rows = B - own.row0 < kMaxRows ? B - own.row0 : kMaxRows;
+            own.ml = reinterpret_cast<float2*>(ws + pl.own_ml) + k * pl.own_slots * kHeads;
+            own.acc = reinterpret_cast<float*>(ws + pl.own_acc) + k * pl.own_slots * kHeads * pv.D;
+            own.before = reinterpret_cast<long long*>(ws + pl.own_before) + (size_t)k * (kMaxRows + 1);
+            if (!launch(part, prefix_ctas(), kOwnWarps * 32, kOwnSmem, n_groups > 0 && k == 0, map, own)) return FPKV_ELAUNCH;
+        }
         const int merge_grid = (pl.tiles * pv.H * (kPrefixTileRows / 32) + (B * Hq + 31) / 32) * (pv.D / 32);
-        return launch(part, B * pv.H * pl.head_blocks * pl.splits, n_groups > 0, own) && launch(merge, merge_grid, true, mrg) ? FPKV_OK : FPKV_ELAUNCH;
+        return launch(merge, merge_grid, 256, 0, true, mrg) ? FPKV_OK : FPKV_ELAUNCH;
     };
     if (pv.dtype == FPKV_BF16)
         return pv.D == 128 ? run(own_part_kernel<__nv_bfloat16, 128>, shared_merge_kernel<__nv_bfloat16, 128>)

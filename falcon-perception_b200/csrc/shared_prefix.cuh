@@ -1,6 +1,7 @@
 // What the two halves of shared-prefix decode attention agree on: rows, groups, and how the prefixes' key tiles are shared out.
 #pragma once
 
+#include <cuda.h>
 #include "common.cuh"
 
 namespace fpkv {
@@ -30,6 +31,8 @@ constexpr int kPrefixTileRows = 128;
 
 int prefix_ctas();
 bool prefix_supported(const PoolView& pv);
+// Tensor map of one layer's K and V planes: `rows` token rows at a time, 64-element column groups one behind the other.
+bool encode_rows(CUtensorMap* map, const PoolView& pv, int layer, int rows);
 int launch_prefix(const PoolView& pv, int layer, const void* q, long long q_stride_b, long long q_stride_h, PrefixParams prm, cudaStream_t stream);
 
 // Visible keys of a row and its slot; a slot or position out of range gives none.

@@ -87,6 +87,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     constexpr int kTileBytesD = kTileM * D * 2;
 
     // ---- set-up: barriers, tensor memory, key tiles before each group -----------------
+    if (warp == kLoadWarp && lane == 0) {                  // the maps themselves come from memory, too
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&q_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kv_map)) : "memory");
+    }
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             bar_init(desc_full0 + 8 * b, 1); bar_init(desc_empty0 + 8 * b, 3 + 2 * kSoftmaxWarps);
@@ -500,21 +504,25 @@ bool prefix_supported(const PoolView& pv)
     return (long long)2 * pv.H * pv.n_pages * pv.P < (1ll << 31);
 }
 
+bool encode_rows(CUtensorMap* map, const PoolView& pv, int layer, int rows)
+{
+    if (encoder() == nullptr) return false;
+    const int halves = pv.D / 64;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)2 * pv.H * pv.n_pages * pv.P, (cuuint64_t)halves};
+    const cuuint64_t strides[2] = {(cuuint64_t)halves * 128, 128};
+    const cuuint32_t box[3] = {64, (cuuint32_t)rows, (cuuint32_t)halves};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return encoder()(map, pv.dtype == FPKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pv.plane(layer, 0, 0), dims,
+                     strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_prefix(const PoolView& pv, int layer, const void* q, long long q_stride_b, long long q_stride_h, PrefixParams prm, cudaStream_t stream)
 {
     if (encoder() == nullptr) return FPKV_EARCH;
     const CUtensorMapDataType dt = pv.dtype == FPKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap kv_map, q_map;
-    {   // one layer's K and V planes: 64-element column groups of token rows, a page at a time
-        const int halves = pv.D / 64;
-        const cuuint64_t dims[3] = {64, (cuuint64_t)2 * pv.H * pv.n_pages * pv.P, (cuuint64_t)halves};
-        const cuuint64_t strides[2] = {(cuuint64_t)halves * 128, 128};
-        const cuuint32_t box[3] = {64, (cuuint32_t)kPage, (cuuint32_t)halves};
-        const cuuint32_t es[3] = {1, 1, 1};
-        if (encoder()(&kv_map, dt, 3, pv.plane(layer, 0, 0), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return FPKV_ELAUNCH;
-    }
+    if (!encode_rows(&kv_map, pv, layer, kPage)) return FPKV_ELAUNCH;
     {   // queries (head_dim, heads, rows): a box of 64 elements x n_rep heads x the rows of a tile is a block of 128-byte rows
         const RowParams& rp = prm.rows;
         prm.q_box_rows = rp.rows_per_tile * rp.n_rep;
