@@ -400,7 +400,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_consta
                     umma_commit(all_done0 + 8 * g);
                     ++wg;
                 } else if (n > 0) {
-                    bar_arrive(q_empty0 + 8 * qb);         // single head, one key tile: nothing for this issuer, only its share of the hand-back
+                    // Single head, one key tile: nothing for this issuer, only its share of the hand-back -- of this item's
+                    // queries, so not before they are there: two items' shares would pass for both issuers' of one.
+                    if (!bar_wait(q_full0 + 8 * qb, wit & 1u, abort_flag)) { alive = false; break; }
+                    bar_arrive(q_empty0 + 8 * qb);
                 }
                 if (n > 0) { gk += n; ++wit; }
                 bar_arrive(desc_empty0 + 8 * b);
