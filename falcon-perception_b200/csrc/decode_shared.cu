@@ -17,8 +17,8 @@
 //    own operand and no access to the ring conflicts.  Bound by the bytes of the rows' own keys.
 //  * merge: joins the partials of every (row, head), applies the sink gate, writes out and lse.
 // The three are chained by programmatic dependent launch: the own part starts as soon as every CTA of the prefix part has
-// (it needs nothing from it) and fills the SMs as they come free; it ends after the prefix part, so that the merge, whose
-// set-up overlaps both, has only the own part to wait for.
+// (it needs nothing from it) and fills the SMs as they come free; it ends after the prefix part, so that the merge has only
+// the own part to wait for.  Both parts write down for the merge which partials belong to whom.
 
 #include "tc5.cuh"
 #include "shared_prefix.cuh"
@@ -44,7 +44,7 @@ struct OwnParams {
     // row, stored head by stored head, 8 query heads by 8 query heads
     float2* ml;
     float* acc;
-    long long* before;                         // [rows + 1] blocks of all segments before a row, for the merge
+    int4* entries;                             // [rows][segments] for the merge: {first slot, partials, group + 1, 0}
     long long q_stride_b, q_stride_h;
     int row0, n_rows, head_blocks;             // the launch's rows; blocks of kHeads query heads of a stored head
     int rows_per_plane;
@@ -52,11 +52,12 @@ struct OwnParams {
 };
 
 struct MergeParams {
-    RowParams rows;
+    const int4* segments;                      // of the prefix part
+    const int4* entries;                       // of the own part
     const float2* pre_ml; const float* pre_acc;
-    const float2* own_ml; const float* own_acc; const long long* own_before;
+    const float2* own_ml; const float* own_acc;
     size_t own_slots;                          // partials of one launch of the own part
-    int workers, head_blocks, ctas, tiles;     // of the own part; of the prefix part, upper bound of its query tiles
+    int B, Hq, n_rep, head_blocks, n_segments; // n_segments: upper bound, of the prefix part
     void* out;
     float* lse;
     Epilogue epi;
@@ -107,6 +108,7 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_before[kMaxRows + 1];
     __shared__ int s_slot[kMaxRows], s_first[kMaxRows], s_keys[kMaxRows];    // slot, first own page, visible keys of each row
+    __shared__ short s_group[kMaxRows];        // its group + 1, 0 for none
     __shared__ uint64_t s_bars[kOwnWarps][kStages];
     __shared__ int s_abort;
     asm volatile("griddepcontrol.launch_dependents;");       // the merge may take its seats
@@ -124,8 +126,8 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
         const int b = prm.row0 + i;
         int slot; int4 d;
         const int keys = row_keys(rp, b, &slot, blockIdx.x == 0);
-        const int first = group_of_row(rp, b, &d) >= 0 ? d.z : 0;
-        s_slot[i] = slot; s_first[i] = first; s_keys[i] = keys;
+        const int group = group_of_row(rp, b, &d), first = group >= 0 ? d.z : 0;
+        s_slot[i] = slot; s_first[i] = first; s_keys[i] = keys; s_group[i] = (short)(group + 1);
         s_before[i + 1] = (long long)max(0, (keys + kBlock - 1) / kBlock - first * kPageBlocks) * n_segs;
     }
     __syncthreads();
@@ -142,11 +144,22 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
         if (lane == 0) s_before[0] = 0;
     }
     __syncthreads();
-    if (blockIdx.x == 0) for (int i = threadIdx.x; i <= prm.n_rows; i += kOwnWarps * 32) prm.before[i] = s_before[i];
     const long long total = s_before[prm.n_rows];
-    const int workers = sharers(total, gridDim.x * kOwnWarps), me = blockIdx.x * kOwnWarps + warp;
-    long long pos = me < workers ? share_begin(total, me, workers) : 0;
-    const long long end = me < workers ? share_begin(total, me + 1, workers) : 0;
+    const int me = blockIdx.x * kOwnWarps + warp;
+    const long long share = share_size(total, gridDim.x * kOwnWarps), end = min(total, (me + 1) * share);
+    long long pos = min(end, me * share);
+    // the merge's table
+    for (int i = blockIdx.x * kOwnWarps * 32 + threadIdx.x; i < prm.n_rows * n_segs; i += gridDim.x * kOwnWarps * 32) {
+        const int r = i / n_segs, seg = i - r * n_segs;
+        const long long blocks = s_before[r + 1] - s_before[r];
+        int4 e = make_int4(0, 0, s_group[r], 0);
+        if (blocks > 0) {
+            const long long nb = blocks / n_segs, first = s_before[r] + nb * seg;
+            const int w0 = (int)(first / share);
+            e.x = w0 + i; e.y = (int)((first + nb - 1) / share) - w0 + 1;
+        }
+        prm.entries[i] = e;
+    }
 
     // A piece: blocks [blk0, blk0 + n) of a segment.
     struct Piece { int row, first, keys, seg, blk0, n, h; };
@@ -359,57 +372,35 @@ __global__ void __launch_bounds__(256)
 shared_merge_kernel(const MergeParams prm)
 {
     constexpr int kColBlocks = D / 32;
-    const RowParams& rp = prm.rows;
-    __shared__ long long flat_before[FPKV_MAX_GROUPS + 1];
-    __shared__ int mt_before[FPKV_MAX_GROUPS + 1];
     __shared__ float2 s_ml[kMergePieces][32];
     __shared__ float s_half[4][9][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = warp / 4;
     const int col4 = (blockIdx.x % kColBlocks) * 8 + warp % 4 * 2, block = blockIdx.x / kColBlocks;
-    const int tile_blocks = prm.tiles * rp.H * (kPrefixTileRows / 32);
-    int b = -1, hq = 0, c0 = 0, n_pre = 0, index = 0, trow = 0;
+    const int tile_blocks = prm.n_segments * (kPrefixTileRows / 32);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int b = -1, hq = 0, n_pre = 0, slot = 0, trow = 0, group = 0;
     if (block < tile_blocks) {
-        if (warp == 0) prefix_schedule(rp, flat_before, mt_before, lane);
-        __syncthreads();
-        const int quarter = block % (kPrefixTileRows / 32), seg0 = block / (kPrefixTileRows / 32);
-        if (seg0 >= mt_before[rp.n_groups] * rp.H) return;
-        int lo = 0, hi = rp.n_groups;          // the group whose segments (query tiles times stored heads) hold this one
-        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (mt_before[mid] * rp.H <= seg0) lo = mid; else hi = mid; }
-        const int4 d = group_at(rp, lo);
-        const long long total = flat_before[rp.n_groups], first = flat_before[lo] + (long long)(seg0 - mt_before[lo] * rp.H) * d.z;
-        const Segment sg = segment_at(rp, flat_before, mt_before, first);
-        trow = quarter * 32 + lane;
-        if (quarter * 32 >= sg.rows) return;
-        const int ctas = sharers(total, prm.ctas);
-        c0 = share_of(total, first, ctas);
-        n_pre = share_of(total, first + d.z - 1, ctas) - c0 + 1;
-        index = sg.index;
-        hq = sg.h * rp.n_rep + trow % rp.n_rep;
-        int4 mine;
-        // (a row of the tile that does not name the group has all its keys in its own part)
-        if (trow < sg.rows && group_of_row(rp, sg.b0 + trow / rp.n_rep, &mine) == lo) b = sg.b0 + trow / rp.n_rep;
+        const int4 sg = prm.segments[block / (kPrefixTileRows / 32)];
+        const int rows = sg.y & 255;
+        trow = block % (kPrefixTileRows / 32) * 32 + lane;
+        if (trow < rows) { b = sg.x + trow / prm.n_rep; hq = (sg.y >> 8) * prm.n_rep + trow % prm.n_rep; }
+        slot = sg.z; n_pre = sg.w & 0xffff; group = (sg.w >> 16) + 1;
     } else {
         const int i = (block - tile_blocks) * 32 + lane;
-        int4 mine;
-        if (i < rp.B * rp.Hq && group_of_row(rp, i / rp.Hq, &mine) < 0) { b = i / rp.Hq; hq = i % rp.Hq; }
+        if (i < prm.B * prm.Hq) { b = i / prm.Hq; hq = i % prm.Hq; }
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (__ballot_sync(0xffffffffu, b >= 0) == 0) return;     // the same for all warps
-    // the row's partials of the own part: first slot (times 8, plus the head) and number
+    // the row's partials of the own part: first one (times 8, plus the head) and number
     size_t own = 0;
     int n_own = 0;
     if (b >= 0) {
-        const int chunk = b / kMaxRows, i = b % kMaxRows, rows = min(kMaxRows, rp.B - chunk * kMaxRows);
-        const long long* before = prm.own_before + (size_t)chunk * (kMaxRows + 1);
-        const long long at = before[i], blocks = before[i + 1] - at, total = before[rows];
-        if (blocks > 0) {
-            const int n_segs = rp.H * prm.head_blocks, rep = hq % rp.n_rep, seg = hq / rp.n_rep * prm.head_blocks + rep / kHeads;
-            const long long nb = blocks / n_segs, first = at + nb * seg;
-            const int workers = sharers(total, prm.workers), w0 = share_of(total, first, workers);
-            n_own = share_of(total, first + nb - 1, workers) - w0 + 1;
-            own = ((size_t)chunk * prm.own_slots + (size_t)w0 + (size_t)i * n_segs + seg) * kHeads + rep % kHeads;
-        }
+        const int rep = hq % prm.n_rep, seg = hq / prm.n_rep * prm.head_blocks + rep / kHeads, n_segs = prm.Hq / prm.n_rep * prm.head_blocks;
+        const int4 e = prm.entries[(size_t)b * n_segs + seg];
+        n_own = e.y;
+        own = ((size_t)(b / kMaxRows) * prm.own_slots + e.x) * kHeads + rep % kHeads;
+        if (e.z != group) b = -1;              // a row of the tile that does not name the group, or here a row that is in one
     }
+    if (__ballot_sync(0xffffffffu, b >= 0) == 0) return;     // the same for all warps
+    if (b < 0) n_own = 0;
     const int n = n_pre + (int)__reduce_max_sync(0xffffffffu, (uint32_t)n_own);
     float M = -INFINITY, L = 0.f, a[8];
 #pragma unroll
@@ -422,7 +413,7 @@ shared_merge_kernel(const MergeParams prm)
             const int p = warp + 8 * r, i = p0 + p;
             float2 ml = make_float2(-INFINITY, 0.f);
             if (p < here && b >= 0) {
-                if (i < n_pre) ml = prm.pre_ml[(size_t)(c0 + i + index) * kPrefixTileRows + trow];
+                if (i < n_pre) ml = prm.pre_ml[(size_t)(slot + i) * kPrefixTileRows + trow];
                 else if (i - n_pre < n_own) ml = prm.own_ml[own + (size_t)(i - n_pre) * kHeads];
             }
             s_ml[p][lane] = ml;
@@ -439,7 +430,7 @@ shared_merge_kernel(const MergeParams prm)
         for (int p = half; p < here; p += 2) {
             const float2 ml = s_ml[p][lane];
             const int i = p0 + p;
-            const float4* src = i < n_pre ? reinterpret_cast<const float4*>(prm.pre_acc) + ((size_t)(c0 + i + index) * (D / 4) + col4) * kPrefixTileRows + trow
+            const float4* src = i < n_pre ? reinterpret_cast<const float4*>(prm.pre_acc) + ((size_t)(slot + i) * (D / 4) + col4) * kPrefixTileRows + trow
                                           : reinterpret_cast<const float4*>(prm.own_acc) + (own + (size_t)(i - n_pre) * kHeads) * (D / 4) + col4;
             const size_t step = i < n_pre ? kPrefixTileRows : 1;
             const bool some = ml.y != 0.f;                   // nothing visible: no sums were written
@@ -460,7 +451,7 @@ shared_merge_kernel(const MergeParams prm)
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] += s_half[warp][k][lane];
     L += s_half[warp][8][lane];
-    const size_t row = (size_t)b * rp.Hq + hq;
+    const size_t row = (size_t)b * prm.Hq + hq;
     const float lse = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
     const float gate = sink_gate(prm.epi, hq, lse), inv = L == 0.f ? 0.f : 1.f / L;
     __align__(16) T o[8];
@@ -470,7 +461,7 @@ shared_merge_kernel(const MergeParams prm)
     if (col4 == 0) prm.lse[row] = lse;
 }
 
-struct Plan { int n_rep, rows_per_tile, tiles, head_blocks, workers, chunks; size_t slots, own_slots, pre_ml, pre_acc, own_ml, own_acc, own_before, bytes; };
+struct Plan { int n_rep, rows_per_tile, tiles, head_blocks, workers, chunks; size_t slots, own_slots, pre_ml, pre_acc, own_ml, own_acc, entries, segments, bytes; };
 Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
 {
     Plan p;
@@ -489,7 +480,8 @@ Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
     p.pre_acc = place(p.slots * kPrefixTileRows * pv.D * sizeof(float));
     p.own_ml = place(p.chunks * p.own_slots * kHeads * sizeof(float2));
     p.own_acc = place(p.chunks * p.own_slots * kHeads * pv.D * sizeof(float));
-    p.own_before = place((size_t)p.chunks * (kMaxRows + 1) * sizeof(long long));
+    p.entries = place((size_t)B * pv.H * p.head_blocks * sizeof(int4));
+    p.segments = place((size_t)p.tiles * pv.H * sizeof(int4));
     p.bytes = place(0);
     return p;
 }
@@ -518,6 +510,7 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
     if (n_groups > 0) {
         PrefixParams pre;
         pre.rows = rows; pre.ml = reinterpret_cast<float2*>(ws + pl.pre_ml); pre.acc = reinterpret_cast<float*>(ws + pl.pre_acc);
+        pre.segments = reinterpret_cast<int4*>(ws + pl.segments); pre.max_segments = pl.tiles * pv.H;
         pre.rows_per_plane = 0; pre.q_box_rows = 0; pre.scale_log2 = sm_scale * kLog2e;
         const int rc = launch_prefix(pv, layer, q, qsb, qsh, pre, stream);
         if (rc) return rc;
@@ -526,10 +519,11 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
     own.rows = rows; own.q = q; own.rows_per_plane = pv.n_pages * pv.P;
     own.q_stride_b = qsb; own.q_stride_h = qsh; own.head_blocks = pl.head_blocks; own.scale_log2 = sm_scale * kLog2e;
     MergeParams mrg;
-    mrg.rows = rows; mrg.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); mrg.pre_acc = reinterpret_cast<float*>(ws + pl.pre_acc);
+    mrg.segments = reinterpret_cast<int4*>(ws + pl.segments); mrg.entries = reinterpret_cast<int4*>(ws + pl.entries);
+    mrg.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); mrg.pre_acc = reinterpret_cast<float*>(ws + pl.pre_acc);
     mrg.own_ml = reinterpret_cast<float2*>(ws + pl.own_ml); mrg.own_acc = reinterpret_cast<float*>(ws + pl.own_acc);
-    mrg.own_before = reinterpret_cast<long long*>(ws + pl.own_before); mrg.own_slots = pl.own_slots;
-    mrg.workers = pl.workers; mrg.head_blocks = pl.head_blocks; mrg.ctas = prefix_ctas(); mrg.tiles = pl.tiles;
+    mrg.own_slots = pl.own_slots; mrg.B = B; mrg.Hq = Hq; mrg.n_rep = pl.n_rep; mrg.head_blocks = pl.head_blocks;
+    mrg.n_segments = pl.tiles * pv.H;
     mrg.out = out; mrg.lse = lse; mrg.epi = epi;
     CUtensorMap map;
     if (!encode_rows(&map, pv, layer, kBlock)) return FPKV_ELAUNCH;
@@ -550,7 +544,7 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
             own.row0 = k * kMaxRows; own.n_rows = B - own.row0 < kMaxRows ? B - own.row0 : kMaxRows;
             own.ml = reinterpret_cast<float2*>(ws + pl.own_ml) + k * pl.own_slots * kHeads;
             own.acc = reinterpret_cast<float*>(ws + pl.own_acc) + k * pl.own_slots * kHeads * pv.D;
-            own.before = reinterpret_cast<long long*>(ws + pl.own_before) + (size_t)k * (kMaxRows + 1);
+            own.entries = reinterpret_cast<int4*>(ws + pl.entries) + (size_t)own.row0 * pv.H * pl.head_blocks;
             if (!launch(part, prefix_ctas(), kOwnWarps * 32, kOwnSmem, n_groups > 0 && k == 0, map, own)) return FPKV_ELAUNCH;
         }
         const int merge_grid = (pl.tiles * pv.H * (kPrefixTileRows / 32) + (B * Hq + 31) / 32) * (pv.D / 32);

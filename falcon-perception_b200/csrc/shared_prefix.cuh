@@ -23,6 +23,9 @@ struct PrefixParams {
     RowParams rows;
     float2* ml;                                // partials [slot][128 rows] (m, l): maximum and sum in base 2
     float* acc;                                // [slot][D/4][128 rows][4]
+    int4* segments;                            // [max_segments] for the merge: {first batch row, query rows | stored head << 8, first slot,
+                                               // partials | group << 16}, all zero past the last
+    int max_segments;
     int rows_per_plane, q_box_rows;
     float scale_log2;
 };
@@ -63,16 +66,9 @@ __device__ __forceinline__ int group_of_row(const RowParams& p, int b, int4* d) 
 
 // ---- the schedule: key tiles of all segments in a row -- group by group, head by head, query tile by query tile -- in equal
 // shares.  flat_before[g], mt_before[g]: key tiles (over all segments) and query tiles before group g. --------------------
-// No share is empty: with fewer key tiles than CTAs, the first CTAs have one each.
-__device__ __forceinline__ int sharers(long long total, int ctas) { return (int)min((long long)ctas, total); }
-__device__ __forceinline__ long long share_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
-// The CTA whose share holds a position below the total.
-__device__ __forceinline__ int share_of(long long total, long long pos, int ctas) {
-    int c = (int)min(pos * ctas / total, (long long)(ctas - 1));
-    while (c + 1 < ctas && share_begin(total, c + 1, ctas) <= pos) ++c;
-    while (c > 0 && share_begin(total, c, ctas) > pos) --c;
-    return c;
-}
+// A share is what the fullest one has to hold, so that as few as possible are used: a share more is a partial more, and the
+// fullest one sets the time.
+__device__ __forceinline__ long long share_size(long long total, int sharers) { return total > 0 ? (total + sharers - 1) / sharers : 1; }
 __device__ __forceinline__ void prefix_schedule(const RowParams& p, long long* flat_before, int* mt_before, int lane) {      // one warp
     long long flat = 0;
     int mt = 0;
@@ -117,6 +113,17 @@ __device__ __forceinline__ Segment segment_at(const RowParams& p, const long lon
     const long long slot = p.batch_idx[d.x];
     s.slot0 = slot >= 0 && slot < p.max_batch ? (int)slot : 0;
     return s;
+}
+
+// Segment i of all, as the merge reads it.
+__device__ __forceinline__ int4 segment_entry(const RowParams& p, const long long* flat_before, const int* mt_before, int i, int ctas) {
+    int lo = 0, hi = p.n_groups;               // mt_before[lo] * H <= i < mt_before[hi] * H
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (mt_before[mid] * p.H <= i) lo = mid; else hi = mid; }
+    const int4 d = group_at(p, lo);
+    const int mt = mt_before[lo + 1] - mt_before[lo], in = i - mt_before[lo] * p.H, m = in % mt;
+    const long long share = share_size(flat_before[p.n_groups], ctas), first = flat_before[lo] + (long long)in * d.z;
+    const int c0 = (int)(first / share), b0 = d.x + m * p.rows_per_tile;
+    return make_int4(b0, min(p.rows_per_tile, d.x + d.y - b0) * p.n_rep | (in / mt) << 8, c0 + i, (int)((first + d.z - 1) / share) - c0 + 1 | lo << 16);
 }
 
 }  // namespace fpkv

@@ -116,6 +116,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     __syncthreads();
     tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;");     // the own part needs nothing from here
+    if (warp < 2 * kSoftmaxWarps) {                        // the merge's table, while there are no scores yet
+        const RowParams& rp = prm.rows;
+        const int n_segments = mt_before[rp.n_groups] * rp.H;
+        for (int i = blockIdx.x * 2 * kSoftmaxWarps * 32 + tid; i < prm.max_segments; i += gridDim.x * 2 * kSoftmaxWarps * 32)
+            prm.segments[i] = i < n_segments ? segment_entry(rp, flat_before, mt_before, i, gridDim.x) : make_int4(0, 0, 0, 0);
+    }
     const uint32_t tmem = (uint32_t)*tmem_slot;
     // S/P of side 0 [0,128), of side 1 [128,256), O of side 0 [256,384), of side 1 [384,512)
     bool alive = true;
@@ -125,10 +131,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         // ============================== scout ===================================
         const RowParams& rp = prm.rows;
         const long long total = flat_before[rp.n_groups];
-        const int G = sharers(total, gridDim.x);
-        const bool mine = (int)blockIdx.x < G;
-        long long pos = mine ? share_begin(total, blockIdx.x, G) : 0;
-        const long long end = mine ? share_begin(total, blockIdx.x + 1, G) : 0;
+        const long long share = share_size(total, gridDim.x), end = min(total, (blockIdx.x + 1) * share);
+        long long pos = blockIdx.x * share;
         uint32_t it = 0, ch = 0;
         while (alive) {
             const uint32_t b = it & 1u;
@@ -310,7 +314,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
                     umma_commit(all_done0 + 8 * g);
                     ++wg;
                 } else if (n > 0) {
-                    bar_arrive(q_empty);                   // one key tile: nothing for this side, only its share of the hand-back
+                    // One key tile: nothing for this side, only its share of the hand-back -- of this piece's queries, so not
+                    // before they are there: two pieces' shares would pass for both sides' of one.
+                    if (!bar_wait(q_full, wit & 1u, abort_flag)) { alive = false; break; }
+                    bar_arrive(q_empty);
                 }
                 if (n > 0) { gk += n; ++wit; }
                 bar_arrive(desc_empty0 + 8 * b);

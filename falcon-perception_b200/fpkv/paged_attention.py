@@ -60,7 +60,8 @@ def _epilogue(sinks: Tensor | None, token_major: bool = False):
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)        # torch.cuda.current_stream(device).cuda_stream without the objects
 
 
 @dataclass
@@ -132,6 +133,7 @@ class PagedKVCache(KVCacheBase):
                                    page_size, head_dim, max_batch_size, _DTYPES[dtype], self.split_q_heads)
         self._status = torch.zeros(1, dtype=torch.int32, device=device)
         self._workspace = None
+        self._shared_bytes = {}                     # (rows, query heads, groups) -> scratch of a shared-prefix call
         self.decode_kernel = _lib.DECODE_AUTO       # DECODE_PORTABLE / DECODE_TMA force one kernel
         self.prefill_kernel = _lib.PREFILL_AUTO     # PREFILL_PORTABLE / PREFILL_TC force one kernel
 
@@ -657,17 +659,21 @@ class PagedKVCache(KVCacheBase):
             q = q.contiguous()                      # the kernel's tensor map has no room for a repeated row
         assert shared.groups.is_cuda and shared.groups.is_contiguous() and shared.groups.dtype == torch.int32
         assert shared.row_group.is_cuda and shared.row_group.is_contiguous() and shared.row_group.dtype == torch.int32
-        need = ctypes.c_size_t(0)
-        _lib.check(_lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(self._pool), B, Hq, shared.n_groups,
-                                                               ctypes.byref(need)), "fpkv_decode_shared_workspace_bytes")
+        key = (B, Hq, shared.n_groups)
+        size = self._shared_bytes.get(key)
+        if size is None:
+            need = ctypes.c_size_t(0)
+            _lib.check(_lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(self._pool), B, Hq, shared.n_groups,
+                                                                   ctypes.byref(need)), "fpkv_decode_shared_workspace_bytes")
+            size = self._shared_bytes[key] = need.value
         # scratch of this call alone: from torch's allocator, so that calls on other streams and captured graphs have their own
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
         epi = _epilogue(sinks)
         _lib.check(_lib.lib.fpkv_decode_attn_shared(
             ctypes.byref(self._pool), layer_id, out.data_ptr(), lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
             batch_idx.data_ptr(), input_pos.data_ptr(), _pos_type(input_pos), B, Hq, shared.groups.data_ptr(),
-            shared.n_groups, shared.row_group.data_ptr(), scale, ws.data_ptr(), ws.numel(),
+            shared.n_groups, shared.row_group.data_ptr(), scale, ws.data_ptr(), size,
             ctypes.byref(epi) if epi is not None else None, self._status_ptr(), _stream(self._dev)),
             "fpkv_decode_attn_shared")
 
@@ -698,17 +704,18 @@ class PagedKVCache(KVCacheBase):
             assert tokens.is_cuda, "tensor must be on the cache's CUDA device"
             tokens = tokens.contiguous()
         slots, starts, lens = slots.contiguous(), starts.contiguous(), lens.contiguous()
-        dev = slots.device
-        wide = torch.empty((4 if tokens is not None else 3, 1, L), dtype=torch.int64, device=dev)
-        row, pos, bidx, *ids = wide.unbind(0)
+        dev, planes = slots.device, 4 if tokens is not None else 3
+        wide = torch.empty((planes, 1, L), dtype=torch.int64, device=dev)
         narrow = torch.empty(N * (W + 3) + 1, dtype=torch.int32, device=dev)
-        block, seq, last, off = narrow.split_with_sizes((N * W, N, N, N + 1))
-        out = _lib.FpkvStepOut(ids[0].data_ptr() if ids else None, pos.data_ptr(), bidx.data_ptr(), row.data_ptr(),
-                               block.data_ptr(), seq.data_ptr(), off.data_ptr(), last.data_ptr())
+        a, b, n = wide.data_ptr(), narrow.data_ptr(), 4 * N
+        seq, off = b + n * W, b + n * (W + 2)       # block table, seq_lens, last, offsets
+        out = _lib.FpkvStepOut(a + 24 * L if planes == 4 else None, a + 8 * L, a + 16 * L, a, b, seq, off, seq + n)
         _lib.check(_lib.lib.fpkv_step_tables(
             ctypes.byref(self._pool), slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), N, L, int(align), W,
             tokens.data_ptr() if tokens is not None else None, tokens.numel() if tokens is not None else 0, int(pad_id),
             ctypes.byref(out), self._status_ptr(), _stream(self._dev)), "fpkv_step_tables")
+        row, pos, bidx, *ids = wide.unbind(0)
+        block, seq, last, off = narrow.split_with_sizes((N * W, N, N, N + 1))
         return StepTables(ids[0] if ids else None, pos, bidx, row[0], block.view(N, W), seq, off, last)
 
     def prefill_attention(self, layer_id: int, q: Tensor, batch_idx: Tensor, input_pos: Tensor, mask: PrefillMask,

@@ -76,5 +76,5 @@ def sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float | None =
     _lib.check(_lib.lib.fpkv_sample(
         logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), B, V, uniform.data_ptr(), ptr(temperature), ptr(top_k),
         ptr(top_p), ptr(min_p), token.data_ptr(), logprob.data_ptr(),
-        torch.cuda.current_stream(logits.device).cuda_stream), "fpkv_sample")
+        torch._C._cuda_getCurrentRawStream(logits.device.index)), "fpkv_sample")
     return token, logprob

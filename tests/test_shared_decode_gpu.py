@@ -113,6 +113,7 @@ BATCHES = {
     "odd sizes and spare rows": ([(3, [385, 400, 777]), (1, [200, 128]), (7, [900] * 5)], (1, 128, 129, 1500)),
     "wide group": ([(2, [257 + i for i in range(70)])], (40,)),
     "very wide group": ([(1, [129 + (i % 5) for i in range(150)]), (3, [390] * 3)], ()),
+    "odd shares": ([(53, [53 * 128 + 5 * i + 1 for i in range(3)]), (5, [700, 701]), (1, [140, 300])], (77,)),
     "long prefix": ([(65, [65 * 128 + 1 + 50 * i for i in range(4)])], (9000,)),
 }
 
