@@ -361,21 +361,21 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
     asm volatile("griddepcontrol.wait;" ::: "memory");       // not done before the prefix part is
 }
 
-// Block: 32 (row, head) pairs, one a lane, and 32 columns: four column groups x two halves of the partials, a warp each.  The
+// Block: 32 (row, head) pairs, one a lane, and 64 columns: four column groups x two halves of the partials, a warp each.  The
 // pairs are a quarter of a query tile of the prefix part, whose partials lie side by side; behind those blocks come some for
 // the rows that are in no group.  The weights of all partials are worked out first, in parallel, so that the loads of the sums
 // do not wait for one another.
 constexpr int kMergePieces = 32;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 shared_merge_kernel(const MergeParams prm)
 {
-    constexpr int kColBlocks = D / 32;
+    constexpr int kColBlocks = D / 64;
     __shared__ float2 s_ml[kMergePieces][32];
-    __shared__ float s_half[4][9][32];
+    __shared__ float s_half[4][17][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = warp / 4;
-    const int col4 = (blockIdx.x % kColBlocks) * 8 + warp % 4 * 2, block = blockIdx.x / kColBlocks;
+    const int col4 = (blockIdx.x % kColBlocks) * 16 + warp % 4 * 4, block = blockIdx.x / kColBlocks;
     const int tile_blocks = prm.n_segments * (kPrefixTileRows / 32);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int b = -1, hq = 0, n_pre = 0, slot = 0, trow = 0, group = 0;
@@ -402,9 +402,9 @@ shared_merge_kernel(const MergeParams prm)
     if (__ballot_sync(0xffffffffu, b >= 0) == 0) return;     // the same for all warps
     if (b < 0) n_own = 0;
     const int n = n_pre + (int)__reduce_max_sync(0xffffffffu, (uint32_t)n_own);
-    float M = -INFINITY, L = 0.f, a[8];
+    float M = -INFINITY, L = 0.f, a[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = 0.f;
+    for (int k = 0; k < 16; ++k) a[k] = 0.f;
     for (int p0 = 0; p0 < n; p0 += kMergePieces) {
         const int here = min(kMergePieces, n - p0);
         __syncthreads();
@@ -425,8 +425,8 @@ shared_merge_kernel(const MergeParams prm)
         M = mn;
         L *= alpha;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] *= alpha;
-#pragma unroll 8
+        for (int k = 0; k < 16; ++k) a[k] *= alpha;
+#pragma unroll 4
         for (int p = half; p < here; p += 2) {
             const float2 ml = s_ml[p][lane];
             const int i = p0 + p;
@@ -434,30 +434,34 @@ shared_merge_kernel(const MergeParams prm)
                                           : reinterpret_cast<const float4*>(prm.own_acc) + (own + (size_t)(i - n_pre) * kHeads) * (D / 4) + col4;
             const size_t step = i < n_pre ? kPrefixTileRows : 1;
             const bool some = ml.y != 0.f;                   // nothing visible: no sums were written
-            const float4 x = some ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f), y = some ? src[step] : make_float4(0.f, 0.f, 0.f, 0.f);
             const float w = some ? exp2f(ml.x - M) : 0.f;
             L += ml.y * w;
-            a[0] += w * x.x; a[1] += w * x.y; a[2] += w * x.z; a[3] += w * x.w;
-            a[4] += w * y.x; a[5] += w * y.y; a[6] += w * y.z; a[7] += w * y.w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 x = some ? src[k * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+                a[4 * k] += w * x.x; a[4 * k + 1] += w * x.y; a[4 * k + 2] += w * x.z; a[4 * k + 3] += w * x.w;
+            }
         }
     }
     if (half == 1) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s_half[warp - 4][k][lane] = a[k];
-        s_half[warp - 4][8][lane] = L;
+        for (int k = 0; k < 16; ++k) s_half[warp - 4][k][lane] = a[k];
+        s_half[warp - 4][16][lane] = L;
     }
     __syncthreads();
     if (half == 1 || b < 0) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] += s_half[warp][k][lane];
-    L += s_half[warp][8][lane];
+    for (int k = 0; k < 16; ++k) a[k] += s_half[warp][k][lane];
+    L += s_half[warp][16][lane];
     const size_t row = (size_t)b * prm.Hq + hq;
     const float lse = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
     const float gate = sink_gate(prm.epi, hq, lse), inv = L == 0.f ? 0.f : 1.f / L;
-    __align__(16) T o[8];
+    __align__(16) T o[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = gated_out<T>(a[k] * inv, gate, prm.epi.sinks != nullptr);
-    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(prm.out) + row * D + col4 * 4) = *reinterpret_cast<const uint4*>(o);
+    for (int k = 0; k < 16; ++k) o[k] = gated_out<T>(a[k] * inv, gate, prm.epi.sinks != nullptr);
+    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(prm.out) + row * D + col4 * 4);
+    dst[0] = reinterpret_cast<const uint4*>(o)[0];
+    dst[1] = reinterpret_cast<const uint4*>(o)[1];
     if (col4 == 0) prm.lse[row] = lse;
 }
 
@@ -467,8 +471,8 @@ Plan plan_of(const PoolView& pv, int B, int Hq, int n_groups)
     Plan p;
     p.n_rep = Hq / pv.H;
     p.rows_per_tile = kPrefixTileRows / p.n_rep;
-    // a group leaves at most one tile that is not full
-    p.tiles = n_groups > 0 ? B / p.rows_per_tile + (n_groups < B ? n_groups : B) : 0;
+    // each group's tiles: its rows over the rows of a tile, rounded up
+    p.tiles = n_groups > 0 ? (int)((B + (long long)(n_groups < B ? n_groups : B) * (p.rows_per_tile - 1)) / p.rows_per_tile) : 0;
     p.head_blocks = (p.n_rep + kHeads - 1) / kHeads;
     p.workers = prefix_ctas() * kOwnWarps;
     p.chunks = (B + kMaxRows - 1) / kMaxRows;
@@ -547,7 +551,7 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
             own.entries = reinterpret_cast<int4*>(ws + pl.entries) + (size_t)own.row0 * pv.H * pl.head_blocks;
             if (!launch(part, prefix_ctas(), kOwnWarps * 32, kOwnSmem, n_groups > 0 && k == 0, map, own)) return FPKV_ELAUNCH;
         }
-        const int merge_grid = (pl.tiles * pv.H * (kPrefixTileRows / 32) + (B * Hq + 31) / 32) * (pv.D / 32);
+        const int merge_grid = (pl.tiles * pv.H * (kPrefixTileRows / 32) + (B * Hq + 31) / 32) * (pv.D / 64);
         return launch(merge, merge_grid, 256, 0, true, mrg) ? FPKV_OK : FPKV_ELAUNCH;
     };
     if (pv.dtype == FPKV_BF16)
