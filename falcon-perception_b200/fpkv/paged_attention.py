@@ -592,8 +592,9 @@ class PagedKVCache(KVCacheBase):
             lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=q.device)
         if shared is not None:
             assert shared.row_group.shape == (B,), "the prefix groups are those of another batch"
-            if shared.n_groups and B and self._shared_supported(Hq) and (sm_scale is None or sm_scale > 0):
-                self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared)
+            n_groups = shared.n_groups
+            if n_groups and B and self._shared_supported(Hq) and (sm_scale is None or sm_scale > 0):
+                self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups)
                 return out, lse
         ws = self._get_workspace(B, Hq)
         scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
@@ -653,29 +654,30 @@ class PagedKVCache(KVCacheBase):
         return (self.dtype != torch.float32 and not self.split_q_heads and self.page_size == 128
                 and Hq // self.n_heads <= 16)
 
-    def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared):
-        B, Hq, _, D = q.shape
-        if 0 in (q.stride(0), q.stride(1)):
-            q = q.contiguous()                      # the kernel's tensor map has no room for a repeated row
-        assert shared.groups.is_cuda and shared.groups.is_contiguous() and shared.groups.dtype == torch.int32
-        assert shared.row_group.is_cuda and shared.row_group.is_contiguous() and shared.row_group.dtype == torch.int32
-        key = (B, Hq, shared.n_groups)
+    def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups):
+        stride_b, stride_h = q.stride()[:2]
+        if stride_b == 0 or stride_h == 0:          # the kernel's tensor map has no room for a repeated row
+            q = q.contiguous()
+            stride_b, stride_h = q.stride()[:2]
+        groups, row_group = shared.groups, shared.row_group
+        assert groups.is_cuda and groups.is_contiguous() and groups.dtype is torch.int32, "prefix groups must be int32 on the device"
+        assert row_group.is_cuda and row_group.is_contiguous() and row_group.dtype is torch.int32, "prefix groups must be int32 on the device"
+        key = (B, Hq, n_groups)
         size = self._shared_bytes.get(key)
         if size is None:
             need = ctypes.c_size_t(0)
-            _lib.check(_lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(self._pool), B, Hq, shared.n_groups,
-                                                                   ctypes.byref(need)), "fpkv_decode_shared_workspace_bytes")
+            _lib.check(_lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(self._pool), B, Hq, n_groups, ctypes.byref(need)),
+                       "fpkv_decode_shared_workspace_bytes")
             size = self._shared_bytes[key] = need.value
         # scratch of this call alone: from torch's allocator, so that calls on other streams and captured graphs have their own
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
+        scale = self.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
         epi = _epilogue(sinks)
         _lib.check(_lib.lib.fpkv_decode_attn_shared(
-            ctypes.byref(self._pool), layer_id, out.data_ptr(), lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
-            batch_idx.data_ptr(), input_pos.data_ptr(), _pos_type(input_pos), B, Hq, shared.groups.data_ptr(),
-            shared.n_groups, shared.row_group.data_ptr(), scale, ws.data_ptr(), size,
-            ctypes.byref(epi) if epi is not None else None, self._status_ptr(), _stream(self._dev)),
-            "fpkv_decode_attn_shared")
+            ctypes.byref(self._pool), layer_id, out.data_ptr(), lse.data_ptr(), q.data_ptr(), stride_b, stride_h,
+            batch_idx.data_ptr(), input_pos.data_ptr(), _pos_type(input_pos), B, Hq, groups.data_ptr(), n_groups,
+            row_group.data_ptr(), scale, ws.data_ptr(), size, ctypes.byref(epi) if epi is not None else None,
+            self._status_ptr(), _stream(self._dev)), "fpkv_decode_attn_shared")
 
     # ------------------------------------------------------------- step indices
     def step_tables(self, slots: Tensor, starts: Tensor, lens: Tensor, row_tokens: int, width: int | None = None,
@@ -691,19 +693,21 @@ class PagedKVCache(KVCacheBase):
         back to back.  ``width``: columns of the block table (default: n_pages).
         The result feeds ``insert_kv``, ``pre_attention_append`` and
         ``prefill_attention``."""
-        assert slots.ndim == 1 and starts.shape == slots.shape and lens.shape == slots.shape, "one slot, start and length a request"
-        assert slots.dtype == torch.int64, "slots must be int64"
-        assert starts.dtype == torch.int32 and lens.dtype == torch.int32, "starts and lens must be int32"
-        assert tokens is None or (tokens.dtype == torch.int64 and tokens.ndim == 1), "tokens must be one int64 row"
-        N, L = slots.shape[0], int(row_tokens)
+        N, L = slots.numel(), int(row_tokens)
+        assert slots.ndim == starts.ndim == lens.ndim == 1 and starts.numel() == N == lens.numel(), "one slot, start and length a request"
+        assert slots.dtype is torch.int64, "slots must be int64"
+        assert starts.dtype is torch.int32 and lens.dtype is torch.int32, "starts and lens must be int32"
+        assert tokens is None or (tokens.dtype is torch.int64 and tokens.ndim == 1), "tokens must be one int64 row"
         W = self.n_pages if width is None else int(width)
         assert L >= 0 and W >= 0 and align > 0, "row_tokens, width and align must not be negative"
         assert N <= _lib.MAX_REQUESTS, f"more than {_lib.MAX_REQUESTS} requests"
         self._require_cuda(slots, starts, lens)
         if tokens is not None:
             assert tokens.is_cuda, "tensor must be on the cache's CUDA device"
-            tokens = tokens.contiguous()
-        slots, starts, lens = slots.contiguous(), starts.contiguous(), lens.contiguous()
+            if not tokens.is_contiguous():
+                tokens = tokens.contiguous()
+        if not (slots.is_contiguous() and starts.is_contiguous() and lens.is_contiguous()):
+            slots, starts, lens = slots.contiguous(), starts.contiguous(), lens.contiguous()
         dev, planes = slots.device, 4 if tokens is not None else 3
         wide = torch.empty((planes, 1, L), dtype=torch.int64, device=dev)
         narrow = torch.empty(N * (W + 3) + 1, dtype=torch.int32, device=dev)

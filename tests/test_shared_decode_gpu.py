@@ -127,6 +127,15 @@ def test_against_64_bits(shape, batch):
     check(out, lse, reference(c, 0, q, slots, last), batch)
 
 
+@pytest.mark.parametrize("batch", [([(1, [129 + i % 40 for i in range(600)]), (1, [128 + i % 300 for i in range(480)])], (1, 300)),
+                                   ([(1 + g % 3, [500, 400 + g]) for g in range(70)], ())], ids=["more rows than a launch", "many groups"])
+def test_large_batches(batch):
+    c, slots, last, q = build(4, 2, 64, torch.bfloat16, *batch)
+    out, lse, g = run(c, slots, last, q)
+    assert g.n_groups == len(batch[0])
+    check(out, lse, reference(c, 0, q, slots, last))
+
+
 def test_agrees_with_the_unshared_path_and_the_call_site():
     c, slots, last, q = build(16, 8, 128, torch.bfloat16, *BATCHES["odd sizes and spare rows"], layers=3, layer=2)
     bi, ip = torch.tensor(slots, device="cuda"), torch.tensor(last, device="cuda")
