@@ -7,22 +7,25 @@
 // A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary in its shared memory: the logits are
 // read from memory once.  Steps, with a cluster barrier behind each:
 //   1. slices to shared memory (NaN becomes -inf, -0 becomes 0), largest and smallest value
-//   2. top-k: the values down to a bound that at least k entries reach (every thread's largest value reaches the
-//      smallest of them) are counted over 1024 even bins; the bin of the k-th entry is collected and sorted.  If
-//      everything down to that bin fits the list, all of it is collected and the rest of the work is done on the list.
-//   3. top-p: 32-bit sums of the weights over 16 wide bins, private to each thread (atomics on shared memory cost seven
-//      times as much), then counts over 1024 bins of the one in which the border lies; the entries around the border
-//      are collected
+//   2. top-k.  A small k: of every thread's largest value the k-th largest has k entries at or above it and hardly more;
+//      those are collected and sorted, and the first CTA does the rest of the row on that list.  A large k: counts over 1024
+//      even bins, then the entries of the bin of the k-th.
+//   3. top-p: 32-bit sums of the weights over 16 wide bins, private to each thread (atomics of all entries on shared memory
+//      took seven times as long), then counts over 1024 bins around the border; the entries around it are collected
 //   4. weights exp((x - max) / T) in 64 bits and their sums over chunks of the slice; for top-p the collected entries are
 //      sorted and added up behind the exact sum of all larger ones, and the guess of step 3 is checked by it
 //   5. the slice, the chunk and then the entry in which the running sum passes u times the sum
 // A value that more entries share than are collected is narrowed down to and its entries are counted off by index.
-// Where a guess fails all the same, the threshold number is found by bisection, one sum over the slices a step.
+// Where a guess fails all the same, the threshold value is found by bisection, one sum over the slices a step.
 //
-// Weights and sums are 64-bit: the token is the answer, and which one it is may hang on the last bits of a sum over the
-// vocabulary (32-bit sums would draw another token in about one row of a hundred at 65536 flat entries).  The 64-bit
-// pipe has half the lanes of the 32-bit one, so the exponential is the table-and-polynomial one below: 9 operations.
+// Sums are 64-bit and weights good to 1.5e-13: the token is the answer, and which one it is may hang on the last bits of a
+// sum over the vocabulary (32-bit sums would draw another token in about one row of a hundred at 65536 flat entries).  The
+// 64-bit pipe has half the lanes of the 32-bit one, so the exponential is the table-and-polynomial one below: 12 operations.
 // No result depends on the order in which atomics arrive: counts are integers, collected entries are sorted.
+//
+// What bounds it: a few rows (1 x 65536 with top-p: 34 us) the chain of about ten barriers and lookups; many rows (512 x
+// 131072 in 32 bits, 268 MB, 41 us of memory) the instructions an entry takes: about 15 to load and compare it, 25 for the
+// wide bins, 10 for the counts, 50 for the 64-bit weight.
 
 #include "common.cuh"
 

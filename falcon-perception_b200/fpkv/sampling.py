@@ -50,8 +50,8 @@ def sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float | None =
 
     Returns ``token`` (B,) int64 and ``logprob`` (B,) float32, the logarithm of the
     probability the token was drawn with (0 for greedy rows).  A NaN logit counts
-    as -inf; a row of nothing but -inf gives token -1, logprob -inf.  Weights and
-    sums are 64-bit; the result does not depend on how the row was split up."""
+    as -inf; a row of nothing but -inf gives token -1, logprob -inf.  Sums are
+    64-bit and weights good to 2e-13, whatever the type of the logits."""
     assert logits.ndim == 2, "logits must be (rows, vocabulary)"
     assert logits.dtype in _DTYPES, "logits must be float32, bfloat16 or float16"
     B, V = logits.shape

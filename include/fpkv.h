@@ -485,7 +485,7 @@ FPKV_API int fpkv_step_tables(const fpkv_pool* pool, const int64_t* slots, const
  *   token   = the first kept index, in vocabulary order, at which the running sum
  *             of the kept w exceeds uniform * their sum;
  *   logprob = log(w_token / sum of the kept w).
- * All of this in 64 bits (48 at least), whatever the type of the logits.
+ * Sums are in 64 bits and weights good to 2e-13, whatever the type of the logits.
  *   logits       device (rows, vocab) of `dtype`, rows row_stride elements apart,
  *                vocab contiguous; aligned to its element size
  *   uniform      device float [rows], in [0, 1)

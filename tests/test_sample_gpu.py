@@ -211,3 +211,15 @@ def test_captured_with_new_inputs():
 def test_no_rows():
     tok, lp = sample(torch.zeros(0, 100, device="cuda"), torch.zeros(0, device="cuda"))
     assert tok.shape == (0,) and lp.shape == (0,)
+
+
+@pytest.mark.parametrize("shape,dtype", [((2, 600001), torch.float32), ((1, 2097153), torch.bfloat16)], ids=["600001-fp32", "2097153-bf16"])
+def test_rows_too_long_for_shared_memory(shape, dtype):
+    """Slices that do not fit on chip are read again in every step."""
+    B, V = shape
+    g = gen(V)
+    x = logits_of(B, V, dtype, g)
+    r = torch.rand(3, B, generator=g, device="cuda")
+    for kw in ({}, {"p": r[1].contiguous()}, {"k": torch.full((B,), 5000, dtype=torch.int32, device="cuda"), "mp": 0.01 * r[2]},
+               {"k": torch.full((B,), 40, dtype=torch.int32, device="cuda"), "p": r[1].contiguous()}):
+        check(x, r[0].contiguous(), what=str(kw.keys()), **kw)
