@@ -264,7 +264,8 @@ class SlotState:
     def sample(self, bucket: int, logits: Tensor, uniform: Tensor, temperature=None, top_k=None, top_p=None, min_p=None):
         """Draw every row's next token (``fpkv.sampling.sample``) and move the
         batch on (``advance``).  Device work only, in the order a captured decode
-        step has it.  Returns (token, logprob) of the bucket's rows."""
+        step has it.  Returns (token, logprob) of the bucket's rows.  A row whose
+        logits allow nothing gets token -1: it is for the caller to end it."""
         token, logprob = sample(logits, uniform, temperature, top_k, top_p, min_p)
         self.advance(bucket, token)
         return token, logprob

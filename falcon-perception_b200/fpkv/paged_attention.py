@@ -568,7 +568,8 @@ class PagedKVCache(KVCacheBase):
         rows have in common are read once for all of them; the result is the same.
         Pools that ``fpkv_decode_attn_shared`` does not take (fp32, split layout,
         page sizes other than 128, more than 16 query heads per stored head) are
-        served row by row as without it, as is a scale that is not positive."""
+        served row by row as without it, as are pools of 2^31 or more rows over all
+        heads and a scale that is not positive."""
         B, Hq, S, D = q.shape
         assert S == 1, "decode attention takes one query token per row"
         assert D == self.head_dim and Hq % self.n_heads == 0, "head layout must match the pool"
@@ -593,7 +594,7 @@ class PagedKVCache(KVCacheBase):
         if shared is not None:
             assert shared.row_group.shape == (B,), "the prefix groups are those of another batch"
             n_groups = shared.n_groups
-            if n_groups and B and self._shared_supported(Hq) and (sm_scale is None or sm_scale > 0):
+            if n_groups and B and self._shared_supported(B, Hq) and (sm_scale is None or sm_scale > 0):
                 self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups)
                 return out, lse
         ws = self._get_workspace(B, Hq)
@@ -650,11 +651,16 @@ class PagedKVCache(KVCacheBase):
         flat = flat.to(self._dev)
         return PrefixGroups(flat[:4 * len(found)].view(-1, 4), flat[4 * len(found):])
 
-    def _shared_supported(self, Hq: int) -> bool:
+    def _shared_supported(self, B: int, Hq: int) -> bool:
+        """What ``fpkv_decode_attn_shared`` takes; anything else is served row by row."""
         return (self.dtype != torch.float32 and not self.split_q_heads and self.page_size == 128
-                and Hq // self.n_heads <= 16)
+                and Hq // self.n_heads <= 16 and B * Hq <= 1 << 24
+                and 2 * self.n_heads * self.n_pages * self.page_size < 1 << 31)
 
     def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups):
+        if torch.cuda.current_device() != q.device.index:
+            with torch.cuda.device(q.device):
+                return self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups)
         stride_b, stride_h = q.stride()[:2]
         if stride_b == 0 or stride_h == 0:          # the kernel's tensor map has no room for a repeated row
             q = q.contiguous()
@@ -702,6 +708,9 @@ class PagedKVCache(KVCacheBase):
         assert L >= 0 and W >= 0 and align > 0, "row_tokens, width and align must not be negative"
         assert N <= _lib.MAX_REQUESTS, f"more than {_lib.MAX_REQUESTS} requests"
         self._require_cuda(slots, starts, lens)
+        if torch.cuda.current_device() != slots.device.index:
+            with torch.cuda.device(slots.device):
+                return self.step_tables(slots, starts, lens, row_tokens, width, align, tokens, pad_id)
         if tokens is not None:
             assert tokens.is_cuda, "tensor must be on the cache's CUDA device"
             if not tokens.is_contiguous():

@@ -178,6 +178,23 @@ def test_one_row_groups_and_groups_without_rows():
         check(out, lse, ref, str(groups))
 
 
+def test_one_slot_in_several_rows():
+    """The same slot at several positions: all its pages are shared, its last one partly filled, rows end inside it."""
+    c, slots, last, q = build(16, 8, 128, torch.bfloat16, [], (700, 130))
+    s, p = [slots[0]] * 4 + [slots[1]] * 2, [699, 0, 511, 640, 129, 128]
+    q = q[[0, 0, 0, 0, 1, 1]] * torch.arange(1, 7, device="cuda", dtype=q.dtype).view(6, 1, 1, 1) / 4
+    out, lse, g = run(c, s, p, q)
+    assert g.groups.tolist() == [[0, 4, 6, 0], [4, 2, 2, 0]]
+    check(out, lse, reference(c, 0, q, s, p))
+
+
+def test_no_rows():
+    c, slots, last, q = build(4, 2, 64, torch.bfloat16, [(1, [130, 140])], ())
+    out, lse = c.decode_attention(0, q[:0], torch.zeros(0, dtype=torch.int64, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"),
+                                  shared=c.prefix_groups([]))
+    assert out.shape == (0, 4, 1, 64) and lse.shape == (0, 4, 1)
+
+
 def test_sink_gate_and_scale():
     c, slots, last, q = build(16, 8, 128, torch.bfloat16, [(2, [300, 310])], ())
     bi, ip = torch.tensor(slots, device="cuda"), torch.tensor(last, dtype=torch.int32, device="cuda")
