@@ -223,3 +223,26 @@ def test_rows_too_long_for_shared_memory(shape, dtype):
     for kw in ({}, {"p": r[1].contiguous()}, {"k": torch.full((B,), 5000, dtype=torch.int32, device="cuda"), "mp": 0.01 * r[2]},
                {"k": torch.full((B,), 40, dtype=torch.int32, device="cuda"), "p": r[1].contiguous()}):
         check(x, r[0].contiguous(), what=str(kw.keys()), **kw)
+
+
+def test_lowest_value_masks_and_large_k():
+    """Half of the row masked by the type's lowest value, k beyond what the threads' largest values bound: the even bins over
+    that distance hold all the rest in one, whatever is narrowed down."""
+    g = gen(21)
+    for V, dtype in ((20000, torch.float32), (20001, torch.bfloat16)):
+        x = logits_of(6, V, dtype, g)
+        x.masked_fill_(torch.rand(6, V, generator=g, device="cuda") < 0.5, torch.finfo(dtype).min)
+        u, r = torch.rand(6, generator=g, device="cuda"), torch.rand(6, generator=g, device="cuda")
+        for k in (5000, 9000, V - 1):
+            kt = torch.full((6,), k, dtype=torch.int32, device="cuda")
+            check(x, u, k=kt, what=f"k {k}")
+            check(x, u, k=kt, p=r, what=f"k {k}, p")
+
+
+def test_borders_among_many_equal_values():
+    """16-bit values of a long row come in groups of hundreds, and the border may lie anywhere among them."""
+    g = gen(22)
+    x = logits_of(48, 262144, torch.bfloat16, g)
+    u = torch.rand(48, generator=g, device="cuda")
+    for lo, hi in ((0.5, 0.999), (0.95, 0.96)):
+        check(x, u, p=torch.linspace(lo, hi, 48, device="cuda"), what=f"p {lo} to {hi}")
