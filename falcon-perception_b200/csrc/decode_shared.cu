@@ -110,7 +110,7 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
     __shared__ int s_slot[kMaxRows], s_first[kMaxRows], s_keys[kMaxRows];    // slot, first own page, visible keys of each row
     __shared__ short s_group[kMaxRows];        // its group + 1, 0 for none
     __shared__ uint64_t s_bars[kOwnWarps][kStages];
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_longest;         // s_longest: blocks of the longest segment
     asm volatile("griddepcontrol.launch_dependents;");       // the merge may take its seats
     const uint32_t ring = ((s32(smem_raw) + 1023u) & ~1023u) + warp * kRingBytes, bars = s32(&s_bars[warp][0]);
     if (threadIdx.x == 0) {
@@ -133,20 +133,23 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
     __syncthreads();
     if (warp == 0) {
         long long carry = 0;
+        int longest = 0;
         for (int i0 = 0; i0 < prm.n_rows; i0 += 32) {
             const int i = i0 + lane;
             long long v = i < prm.n_rows ? s_before[i + 1] : 0;
+            longest = max(longest, (int)(v / n_segs));
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += y; }
             if (i < prm.n_rows) s_before[i + 1] = v + carry;
             carry += __shfl_sync(0xffffffffu, v, 31);
         }
-        if (lane == 0) s_before[0] = 0;
+        longest = (int)__reduce_max_sync(0xffffffffu, (uint32_t)longest);
+        if (lane == 0) { s_before[0] = 0; s_longest = longest; }
     }
     __syncthreads();
     const long long total = s_before[prm.n_rows];
     const int me = blockIdx.x * kOwnWarps + warp;
-    const long long share = share_size(total, gridDim.x * kOwnWarps), end = min(total, (me + 1) * share);
+    const long long share = share_size(total, gridDim.x * kOwnWarps, s_longest), end = min(total, (me + 1) * share);
     long long pos = min(end, me * share);
     // the merge's table
     for (int i = blockIdx.x * kOwnWarps * 32 + threadIdx.x; i < prm.n_rows * n_segs; i += gridDim.x * kOwnWarps * 32) {

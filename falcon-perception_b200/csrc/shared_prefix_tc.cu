@@ -71,7 +71,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     ChunkDesc* chunks = reinterpret_cast<ChunkDesc*>(desc + 2);      // [2]
     float2* xch = reinterpret_cast<float2*>(chunks + 2);   // [2][2 groups][128 rows] (m, l)
     long long* flat_before = reinterpret_cast<long long*>(xch + 2 * 2 * kTileM);      // [n_groups + 1]
-    int* mt_before = reinterpret_cast<int*>(flat_before + FPKV_MAX_GROUPS + 1);       // [n_groups + 1]
+    int* mt_before = reinterpret_cast<int*>(flat_before + FPKV_MAX_GROUPS + 1);       // [n_groups + 2]
 
     uint32_t at = s32(bars);
     auto take = [&](int n) { const uint32_t b = at; at += 8 * n; return b; };
@@ -131,7 +131,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         // ============================== scout ===================================
         const RowParams& rp = prm.rows;
         const long long total = flat_before[rp.n_groups];
-        const long long share = share_size(total, gridDim.x), end = min(total, (blockIdx.x + 1) * share);
+        const long long share = share_size(total, gridDim.x, mt_before[rp.n_groups + 1]), end = min(total, (blockIdx.x + 1) * share);
         long long pos = blockIdx.x * share;
         uint32_t it = 0, ch = 0;
         while (alive) {
@@ -498,7 +498,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
 }
 
 constexpr int kSmem = 1024 + (1 + kStagesK + kStagesV) * kTileBytes + 48 * 8 + 16 * 4 + 2 * (int)sizeof(PieceDesc) + 2 * (int)sizeof(ChunkDesc) +
-                      2 * 2 * kTileM * 8 + (FPKV_MAX_GROUPS + 1) * 12;
+                      2 * 2 * kTileM * 8 + (FPKV_MAX_GROUPS + 1) * 12 + 16;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 
 }  // namespace

@@ -313,3 +313,13 @@ def test_device_tables_follow_shares_and_erases():
             np_, ns = c._alloc_counts.tolist()
             assert c._free_pages_dev[:np_].tolist() == c.free_pages and c._free_slots_dev[:ns].tolist() == c.free_batch_idx
             c.check_status()
+
+
+@pytest.mark.parametrize("pages,rows,alone", [(63, 4, 3), (64, 4, 3), (65, 2, 1), (131, 3, 0), (190, 1, 2)])
+def test_few_long_segments(pages, rows, alone):
+    """So few segments that an even share would cut each into more pieces than the bound: one stored head, long single rows."""
+    n = pages * P
+    c, slots, last, q = build(8, 1, 128, torch.bfloat16, [(pages, [n + 1 + 37 * i for i in range(rows)])],
+                              [n - 5 - 211 * i for i in range(alone)], seed=pages)
+    out, lse, _ = run(c, slots, last, q)
+    check(out, lse, reference(c, 0, q, slots, last))
