@@ -387,23 +387,27 @@ sample_kernel(const SampleParams prm)
         const float x_ = fmx - d, slack = 4e-7f * (fabsf(fmx) + d);
         return key_of(__float_as_uint(above ? x_ + slack : x_ - slack));
     };
-    // Fine bins: the images in [k_first, k_last], even in the distance; -1 above them, kFine below.
-    uint32_t k_first = 0, k_last = 0;
+    // Fine bins: the images in [k_first, k_last], even in the distance; -1 above them, kFine below.  With k_split, no bin holds
+    // images on both sides of it: those below it start with bin split_bin.
+    uint32_t k_first = 0, k_last = 0, k_split = 0;
+    int split_bin = 0;
     float start = 0.f, per = 0.f;
     auto span = [&](uint32_t first, uint32_t last) {
-        k_first = first; k_last = last;
+        k_first = first; k_last = last; k_split = 0; split_bin = 0;
         start = distance(bits_of(last));
         per = (float)kFine * 0.999f / fmaxf(distance(bits_of(first)) - start, 1e-30f);
     };
     auto fine_of = [&](uint32_t key) -> int {
         if (key > k_last) return -1;
         if (key < k_first) return kFine;
-        return max(0, min((int)((distance(bits_of(key)) - start) * per), kFine - 1));
+        const int b = max(0, min((int)((distance(bits_of(key)) - start) * per), kFine - 1));
+        return key < k_split ? max(b, split_bin) : b;
     };
     // Smallest image whose fine bin is at most b.
     auto edge = [&](int b) -> uint32_t {
         if (b < 0) return k_last + 1u;
         if (b >= kFine - 1) return b < kFine ? k_first : 0u;
+        if (k_split != 0 && b == split_bin - 1) return k_split;
         const float d = start + (float)(b + 1) / per;
         return first_key([&](uint32_t key) { return fine_of(key) <= b; }, near(d, false), near(d, true));
     };
@@ -723,8 +727,17 @@ sample_kernel(const SampleParams prm)
             return first_key([&](uint32_t key) { return distance(bits_of(key)) <= d; }, near(d, false), near(d, true));
         };
         const float width = 1.f / per_wide;
-        float from_d = (float)wb * width;                // where `mass_before` ends
+        const float from_d = (float)wb * width;          // where `mass_before` ends
         span(wb < kWide - 1 ? at_distance(((float)wb + 1.5f) * width) : low, wb > 0 ? at_distance(((float)wb - 0.5f) * width) - 1u : kmax);
+        // The fine bins are cut where that wide bin starts.  A bin told by its middle to lie before or behind that place may be
+        // a whole class of equal 16-bit values on the wrong side (32 to 79 of them in the rows seen, heavier than those at the
+        // border), and the guess then misses: 11 rows in 3840 went to the bisection, and 10 batches of 60 (64 rows of 65536,
+        // bf16) took 300 us instead of 64; none does with the cut.
+        if (wb > 0) {
+            const uint32_t at = first_key([&](uint32_t key) { return wide_of(key) < wb; }, near(from_d, false), near(from_d, true));
+            const int b = at > k_last ? -1 : fine_of(at);
+            if (b < kFine - 1) { split_bin = b + 1; k_split = b < 0 ? 0u : at; }
+        }
         for (int turn = 0; turn < 4; ++turn) {
             count([&] { count_entries(threshold); });
             if (tid == 0) { sh.at[0] = sh.at[3] = kFine; sh.at[4] = sh.at[7] = sh.at[8] = sh.at[10] = -1; sh.at[6] = sh.at[9] = sh.at[11] = 0; }
@@ -732,7 +745,7 @@ sample_kernel(const SampleParams prm)
             const float d0 = start + ((float)(2 * tid) + 0.5f) / per, d1 = start + ((float)(2 * tid) + 1.5f) / per;
             const float m0 = c0 ? (float)c0 * exp2f(-d0 * fslope) : 0.f, m1 = c1 ? (float)c1 * exp2f(-d1 * fslope) : 0.f;
             float total;
-            const float extra = block_sum((d0 < from_d ? m0 : 0.f) + (d1 < from_d ? m1 : 0.f), reinterpret_cast<float*>(sh.red_u));
+            const float extra = block_sum((2 * tid < split_bin ? m0 : 0.f) + (2 * tid + 1 < split_bin ? m1 : 0.f), reinterpret_cast<float*>(sh.red_u));
             const float m_before = mass_before - extra + block_scan(m0 + m1, reinterpret_cast<float*>(sh.red_u), &total) - m0 - m1;
             // one atomic a warp: hundreds on one address take longer than all the rest of this
             const int here = c0 && m_before + m0 >= goal ? 2 * tid : c1 && m_before + m0 + m1 >= goal ? 2 * tid + 1 : kFine;
@@ -774,7 +787,6 @@ sample_kernel(const SampleParams prm)
             lost = tie == 0 && turn == 3;
             if (tie != 0 || lost) break;
             mass_before = __int_as_float(sh.at[5]);
-            from_d = 0.f;
             span(edge(j), edge(j - 1) - 1u);
         }
     }
