@@ -126,7 +126,9 @@ own_part_kernel(const __grid_constant__ CUtensorMap map, const OwnParams prm)
         const int b = prm.row0 + i;
         int slot; int4 d;
         const int keys = row_keys(rp, b, &slot, blockIdx.x == 0);
-        const int group = group_of_row(rp, b, &d), first = group >= 0 ? d.z : 0;
+        int group = group_of_row(rp, b, &d);
+        if (group >= 0 && !slot_maps_pages(rp, slot)) group = -1;
+        const int first = group >= 0 ? d.z : 0;
         s_slot[i] = slot; s_first[i] = first; s_keys[i] = keys; s_group[i] = (short)(group + 1);
         s_before[i + 1] = (long long)max(0, (keys + kBlock - 1) / kBlock - first * kPageBlocks) * n_segs;
     }

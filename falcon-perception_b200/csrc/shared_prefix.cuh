@@ -64,6 +64,23 @@ __device__ __forceinline__ int group_of_row(const RowParams& p, int b, int4* d) 
     return (d->y > 0 && b >= d->x && b < d->x + d->y) ? g : -1;
 }
 
+// Whether a slot maps pages at all: padding (slot 0) and erased slots do not.  Such a row of a group -- a request that has ended
+// since the groups were made -- is as good as in none, and the pages are read through another row's table.
+__device__ __forceinline__ bool slot_maps_pages(const RowParams& p, long long slot) {
+    if (slot <= 0 || slot >= p.max_batch) return false;
+    const long long page = p.page_table[slot * p.n_pages];
+    return page >= 0 && page < p.n_pages;
+}
+// Slot of the first of `rows` batch rows from b0 on that maps pages, 0 if none does.  One warp.
+__device__ __forceinline__ int mapping_slot(const RowParams& p, int b0, int rows, int lane) {
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+        const long long slot = r0 + lane < rows ? p.batch_idx[b0 + r0 + lane] : 0;
+        const uint32_t maps = __ballot_sync(0xffffffffu, slot_maps_pages(p, slot));
+        if (maps) return (int)__shfl_sync(0xffffffffu, slot, __ffs(maps) - 1);
+    }
+    return 0;
+}
+
 // ---- the schedule: key tiles of all segments in a row -- group by group, head by head, query tile by query tile -- in equal
 // shares.  flat_before[g], mt_before[g]: key tiles (over all segments) and query tiles before group g; mt_before[n_groups + 1]:
 // the longest segment's key tiles. --------------------
@@ -104,7 +121,7 @@ struct Segment {
     int index;                                 // over all groups
     int b0, rows, h;                           // first batch row, query rows, stored head
     int pages, tile;                           // key tiles of the segment; the one at the position asked for
-    int slot0;                                 // slot whose table names the pages
+    int group_b0, group_rows;                  // the group's batch rows
 };
 __device__ __forceinline__ Segment segment_at(const RowParams& p, const long long* flat_before, const int* mt_before, long long pos) {
     int lo = 0, hi = p.n_groups;               // flat_before[lo] <= pos < flat_before[hi]
@@ -120,8 +137,7 @@ __device__ __forceinline__ Segment segment_at(const RowParams& p, const long lon
     s.index = mt_before[lo] * p.H + seg;
     s.b0 = d.x + m * p.rows_per_tile;
     s.rows = min(p.rows_per_tile, d.x + d.y - s.b0) * p.n_rep;
-    const long long slot = p.batch_idx[d.x];
-    s.slot0 = slot >= 0 && slot < p.max_batch ? (int)slot : 0;
+    s.group_b0 = d.x; s.group_rows = d.y;
     return s;
 }
 

@@ -151,8 +151,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = lane + 32 * r;
-                int slot;
-                const int n = row < sg.rows ? row_keys(rp, sg.b0 + row / rp.n_rep, &slot, false) : 0;
+                int slot = 0;
+                int n = row < sg.rows ? row_keys(rp, sg.b0 + row / rp.n_rep, &slot, false) : 0;
+                if (!slot_maps_pages(rp, slot)) n = 0;
                 ex[r] = max(0, min(n, sg.pages * kPage) - key0);
                 d->extent[row] = ex[r];
                 emax = max(emax, ex[r]);
@@ -167,7 +168,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
             if (lane == 0) bar_arrive(desc_full0 + 8 * b);
             ++it;
             // pool rows of its key tiles
-            const long long trow = (long long)sg.slot0 * rp.n_pages;
+            const long long trow = (long long)mapping_slot(rp, sg.group_b0, sg.group_rows, lane) * rp.n_pages;
             for (int j0 = 0; j0 < n_tiles && alive; j0 += kChunk, ++ch) {
                 const uint32_t cb = ch & 1u;
                 long long pg[2];

@@ -403,10 +403,12 @@ FPKV_API int fpkv_decode_attn_static(const fpkv_pool* pool, int32_t layer,
  *   groups     device int32 [n_groups][4], 16-byte aligned, each {first row, rows,
  *              shared pages, 0}: batch rows first .. first+rows-1 all map logical
  *              pages 0 .. shared-1 to the same physical pages (the kernel reads
- *              them through the first row's slot).  Groups do not overlap; one
- *              with no rows or no shared pages is skipped.
+ *              them through the slot of the group's first row that maps any).
+ *              Groups do not overlap; one with no rows or no shared pages is
+ *              skipped.
  *   row_group  device int32 [B]: the group of every row, -1 for none.  A row whose
- *              entry does not name a group that contains it counts as in none.
+ *              entry does not name a group that contains it, or whose slot is 0,
+ *              out of range or without pages, counts as in none.
  * Both are device data: a captured call may be replayed with other contents.
  * A row's position may lie anywhere, inside the shared prefix too.  Keys of an
  * unmapped page are not visible, as in fpkv_decode_attn.

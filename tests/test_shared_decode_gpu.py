@@ -323,3 +323,27 @@ def test_few_long_segments(pages, rows, alone):
                               [n - 5 - 211 * i for i in range(alone)], seed=pages)
     out, lse, _ = run(c, slots, last, q)
     check(out, lse, reference(c, 0, q, slots, last))
+
+
+@pytest.mark.parametrize("how", ["padding", "erased", "out of range"])
+@pytest.mark.parametrize("rows,gone", [(4, [0]), (4, [0, 1, 2]), (4, [2]), (3, [0, 1, 2]), (70, list(range(40)))],
+                         ids=["first", "all but the last", "middle", "all", "more than a warp looks at"])
+def test_rows_that_have_ended(how, rows, gone):
+    """Rows of a group whose request ended after the groups were made: nothing for them, whichever they are, and the others keep the
+    prefix, also where it was named by one that has ended."""
+    c, slots, last, q = build(4, 2, 64, torch.bfloat16, [(3, [390 + i for i in range(rows)]), (1, [200, 201])], (300,), seed=rows)
+    g = c.prefix_groups(slots)
+    want = [0 if b in gone else s for b, s in enumerate(slots)]
+    if how == "erased":
+        for b in gone:
+            c.erase(slots[b])
+        now = slots
+    else:
+        now = [s if b not in gone else (0 if how == "padding" else c.max_batch_size + b) for b, s in enumerate(slots)]
+    bi, ip = torch.tensor(now, device="cuda"), torch.tensor(last, dtype=torch.int32, device="cuda")
+    out, lse = c.decode_attention(0, q, bi, ip, shared=g)
+    if how == "out of range":
+        with pytest.raises(RuntimeError, match="bad slot"):
+            c.check_status()
+    c.check_status()
+    check(out, lse, reference(c, 0, q, want, last), how)
