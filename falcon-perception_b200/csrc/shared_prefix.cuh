@@ -83,7 +83,8 @@ __device__ __forceinline__ int mapping_slot(const RowParams& p, int b0, int rows
 
 // ---- the schedule: key tiles of all segments in a row -- group by group, head by head, query tile by query tile -- in equal
 // shares.  flat_before[g], mt_before[g]: key tiles (over all segments) and query tiles before group g; mt_before[n_groups + 1]:
-// the longest segment's key tiles. --------------------
+// the longest segment's key tiles.  The workspace has room for max_tiles query tiles, all that groups without common rows can
+// have; groups are device data, so what does not fit that is left out, and said in the status. --------------------
 // A share is what the fullest one has to hold, so that as few as possible are used: a share more is a partial more, and the
 // fullest one sets the time.  Nor is the longest segment cut into more than kMaxPieces, because the merge goes through a row's
 // partials one after the other.  Whole call, 8 query heads over one stored head of 128, bf16, at most 64 pieces against no bound:
@@ -94,7 +95,7 @@ constexpr int kMaxPieces = 64;
 __device__ __forceinline__ long long share_size(long long total, int sharers, int longest) {
     return max(max((total + sharers - 1) / sharers, (long long)(longest + kMaxPieces - 1) / kMaxPieces), 1ll);
 }
-__device__ __forceinline__ void prefix_schedule(const RowParams& p, long long* flat_before, int* mt_before, int lane) {      // one warp
+__device__ __forceinline__ void prefix_schedule(const RowParams& p, int max_tiles, long long* flat_before, int* mt_before, int lane) {      // one warp
     long long flat = 0;
     int mt = 0, longest = 0;
     for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
@@ -109,6 +110,13 @@ __device__ __forceinline__ void prefix_schedule(const RowParams& p, long long* f
             const long long yf = __shfl_up_sync(0xffffffffu, f, o);
             const int ym = __shfl_up_sync(0xffffffffu, m, o);
             if (lane >= o) { f += yf; m += ym; }
+        }
+        const int fit = __popc(__ballot_sync(0xffffffffu, mt + m <= max_tiles));     // a leading run of the lanes
+        if (fit < 32) {
+            const long long last_f = __shfl_sync(0xffffffffu, f, max(fit - 1, 0));
+            const int last_m = __shfl_sync(0xffffffffu, m, max(fit - 1, 0));
+            if (lane >= fit) { f = fit > 0 ? last_f : 0; m = fit > 0 ? last_m : 0; }
+            if (lane == 0) raise_status(p.status, FPKV_STATUS_BAD_SLOT);
         }
         if (g < p.n_groups) { flat_before[g + 1] = flat + f; mt_before[g + 1] = mt + m; }
         flat += __shfl_sync(0xffffffffu, f, 31);

@@ -111,7 +111,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(tmem_slot)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == kScoutWarp) prefix_schedule(prm.rows, flat_before, mt_before, lane);
+    if (warp == kScoutWarp) prefix_schedule(prm.rows, prm.max_segments / prm.rows.H, flat_before, mt_before, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

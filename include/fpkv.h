@@ -404,8 +404,10 @@ FPKV_API int fpkv_decode_attn_static(const fpkv_pool* pool, int32_t layer,
  *              shared pages, 0}: batch rows first .. first+rows-1 all map logical
  *              pages 0 .. shared-1 to the same physical pages (the kernel reads
  *              them through the slot of the group's first row that maps any).
- *              Groups do not overlap; one with no rows or no shared pages is
- *              skipped.
+ *              Groups have no rows in common (where they do and together need more
+ *              of the workspace than groups without common rows could, some are
+ *              left out, their rows lose the prefix, and FPKV_STATUS_BAD_SLOT is
+ *              raised); one with no rows or no shared pages is skipped.
  *   row_group  device int32 [B]: the group of every row, -1 for none.  A row whose
  *              entry does not name a group that contains it, or whose slot is 0,
  *              out of range or without pages, counts as in none.

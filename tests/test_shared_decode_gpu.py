@@ -1,5 +1,6 @@
 """GPU: decode attention of a batch that shares prefixes, against a 64-bit computation over every row's own keys."""
 
+import ctypes
 import math
 
 import pytest
@@ -347,3 +348,29 @@ def test_rows_that_have_ended(how, rows, gone):
             c.check_status()
     c.check_status()
     check(out, lse, reference(c, 0, q, want, last), how)
+
+
+@pytest.mark.parametrize("n", [100, 128, 1000])
+def test_groups_with_common_rows_stay_inside_the_workspace(n):
+    """Every group names all rows: two query tiles each, twice as many in all as the workspace has room for."""
+    c, slots, last, q = build(4, 2, 64, torch.bfloat16, [(2, [257 + i for i in range(100)])], ())
+    B, H = 100, 2
+    bi, ip = torch.tensor(slots, device="cuda"), torch.tensor(last, dtype=torch.int32, device="cuda")
+    groups = torch.tensor([[0, B, 2, 0]] * n, dtype=torch.int32, device="cuda")
+    row_group = torch.zeros(B, dtype=torch.int32, device="cuda")
+    out, lse = torch.empty(B, 4, 1, 64, dtype=q.dtype, device="cuda"), torch.empty(B, 4, 1, device="cuda")
+    c.flush_tables()
+    need = ctypes.c_size_t(0)
+    assert _lib.lib.fpkv_decode_shared_workspace_bytes(ctypes.byref(c._pool), B, 4, n, ctypes.byref(need)) == 0
+    behind = 64 << 20                                    # more than all the tiles named could write
+    ws = torch.full((need.value + behind,), 0x5a, dtype=torch.uint8, device="cuda")
+    rc = _lib.lib.fpkv_decode_attn_shared(ctypes.byref(c._pool), 0, out.data_ptr(), lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
+                                          bi.data_ptr(), ip.data_ptr(), _lib.FPKV_I32, B, 4, groups.data_ptr(), n, row_group.data_ptr(),
+                                          0.125, ws.data_ptr(), need.value, None, c._status.data_ptr(),
+                                          torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert (ws[need.value:] == 0x5a).all()
+    with pytest.raises(RuntimeError, match="bad slot"):
+        c.check_status()
+    check(out, lse, reference(c, 0, q, slots, last, 0.125))          # their group is the first one, which fits
