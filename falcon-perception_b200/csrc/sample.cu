@@ -269,7 +269,8 @@ sample_kernel(const SampleParams prm)
     const float p_top = prm.top_p != nullptr ? prm.top_p[row] : 1.f;
     const int k_top = prm.top_k != nullptr ? prm.top_k[row] : 0;
     const float p_min = prm.min_p != nullptr ? prm.min_p[row] : 0.f;
-    const double u = (double)prm.uniform[row];
+    // A goal below zero would end the search in a slice, or chunk, without any kept entry.  NaN gives 0 too.
+    const double u = fmax((double)prm.uniform[row], 0.0);
     unsigned long long best = 0;
     uint32_t low = 0xffffffffu, bound = 0xffffffffu;
     uint32_t top = 0;                                    // image of this thread's largest value

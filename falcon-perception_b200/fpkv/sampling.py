@@ -37,7 +37,8 @@ def _per_row(value, name: str, rows: int, dtype: torch.dtype, like: Tensor) -> T
 def sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float | None = None, top_k: Tensor | int | None = None,
            top_p: Tensor | float | None = None, min_p: Tensor | float | None = None) -> tuple[Tensor, Tensor]:
     """One token a row.  ``logits`` (B, V) in fp32, bf16 or fp16 on a CUDA device
-    (rows may be strided); ``uniform`` (B,) float32 in [0, 1).  The settings are
+    (rows may be strided); ``uniform`` (B,) float32 in [0, 1) (below it or NaN
+    counts as 0, beyond it draws the last kept entry).  The settings are
     one number for all rows or one a row: ``temperature`` (<= 0: greedy, the
     lowest index among equal logits), ``top_k`` (<= 0: no limit), ``top_p`` (>= 1:
     no limit), ``min_p`` (<= 0: no limit).

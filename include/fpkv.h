@@ -492,7 +492,8 @@ FPKV_API int fpkv_step_tables(const fpkv_pool* pool, const int64_t* slots, const
  * Sums are in 64 bits and weights good to 2e-13, whatever the type of the logits.
  *   logits       device (rows, vocab) of `dtype`, rows row_stride elements apart,
  *                vocab contiguous; aligned to its element size
- *   uniform      device float [rows], in [0, 1)
+ *   uniform      device float [rows], in [0, 1).  < 0 or NaN counts as 0, >= 1
+ *                draws the last kept entry with any weight
  *   temperature  device float [rows] or NULL (1).  <= 0 or NaN: greedy, logprob 0
  *   top_k        device int32 [rows] or NULL.  <= 0: no limit
  *   top_p        device float [rows] or NULL.  >= 1 or NaN: no limit; <= 0: one entry

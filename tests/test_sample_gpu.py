@@ -246,3 +246,19 @@ def test_borders_among_many_equal_values():
     u = torch.rand(48, generator=g, device="cuda")
     for lo, hi in ((0.5, 0.999), (0.95, 0.96)):
         check(x, u, p=torch.linspace(lo, hi, 48, device="cuda"), what=f"p {lo} to {hi}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("V", [300, 5000, 65536, 600001])
+def test_uniform_numbers_out_of_range(V, dtype):
+    """Below 0 and NaN count as 0.  The kept entries lie at the row's end, behind slices and chunks that hold none."""
+    g = gen(V)
+    x = logits_of(4, V, dtype, g)
+    x[1:, :-20] = -math.inf
+    x[2, -20:] = 2.0
+    for uv in (-1e-30, -0.25, -math.inf, math.nan):
+        for kw in ({}, {"top_p": 0.8}, {"top_k": 7}, {"top_k": 7, "top_p": 0.8}, {"min_p": 0.2}):
+            got = sample(x, torch.full((4,), uv, device="cuda"), **kw)
+            want = sample(x, torch.zeros(4, device="cuda"), **kw)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (uv, kw)
+            assert (got[0] >= 0).all() and (got[0] < V).all() and (got[0][1:] >= V - 20).all()
