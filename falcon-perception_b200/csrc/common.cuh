@@ -93,6 +93,14 @@ __device__ __forceinline__ T gated_out(float o, float gate, bool on) {
     return on ? ElemTraits<T>::from_float(ElemTraits<T>::to_float(r) * gate) : r;
 }
 
+// The code of a launch or of what prepares it.  A refusal is answered here and taken off the thread's last error, where the
+// next call that asks for that would find it.
+inline int launch_code(cudaError_t err) {
+    if (err == cudaSuccess) return FPKV_OK;
+    cudaGetLastError();
+    return FPKV_ELAUNCH;
+}
+
 // ---- launchers implemented in the .cu files (host side, internal) ----------
 int launch_append(const PoolView& pv, int layer, const int64_t* batch_idx, const void* pos, int pos_type,
                   const void* k, long long k_stride_tok, long long k_stride_h,

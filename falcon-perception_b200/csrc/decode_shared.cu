@@ -538,14 +538,14 @@ int launch_decode_shared(const PoolView& pv, int layer, void* out, float* lse, c
     if (!encode_rows(&map, pv, layer, kBlock)) return FPKV_ELAUNCH;
     constexpr int kOwnSmem = 1024 + kOwnWarps * kRingBytes;
     auto launch = [&](auto kern, int grid, int threads, int smem, bool chained, const auto&... args) {
-        if (smem > 0 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+        if (smem > 0 && launch_code(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return false;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr.val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = &attr; cfg.numAttrs = chained ? 1 : 0;
-        return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
+        return launch_code(cudaLaunchKernelEx(&cfg, kern, args...)) == FPKV_OK;
     };
     auto run = [&](auto part, auto merge) {
         // (launches of further rows wait for the one before: each ends after the prefix part, and so after all of its own kind)

@@ -40,6 +40,7 @@ constexpr int kCand = kThreads;                          // entries collected an
 constexpr int kAround = 64;                              // entries collected on either side of the top-p border
 constexpr int kMaxChunks = kThreads;                     // chunks of a slice, one thread each in the final search
 constexpr int kMaxCluster = 8;
+constexpr int kMaxSmem = 220 * 1024;
 constexpr uint32_t kKeyNone = 0x007fffffu;               // image of -inf: never drawn
 
 struct SampleParams {
@@ -1005,7 +1006,7 @@ int launch_typed(SampleParams prm, int rows, cudaStream_t stream)
     // as a slice has to be small for two CTAs to share an SM.
     int cluster = 1;
     while (cluster < kMaxCluster && (long long)prm.vocab > 4096ll * cluster && (long long)rows * cluster * 2 <= 2 * 148) cluster *= 2;
-    const int half = 113 * 1024 - (int)sizeof(Shared), budget = 220 * 1024 - (int)sizeof(Shared);
+    const int half = 113 * 1024 - (int)sizeof(Shared), budget = kMaxSmem - (int)sizeof(Shared);
     auto shape = [&](int c) {
         prm.chunk_vecs = 32;
         while ((long long)prm.chunk_vecs * kMaxChunks * c < row_vecs) prm.chunk_vecs *= 2;
@@ -1017,14 +1018,16 @@ int launch_typed(SampleParams prm, int rows, cudaStream_t stream)
     const bool staged = (long long)prm.slice_vecs * 16 <= budget;
     const int bytes = (int)sizeof(Shared) + (staged ? prm.slice_vecs * 16 : 0);
     auto kern = staged ? sample_kernel<T, true> : sample_kernel<T, false>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return FPKV_ELAUNCH;
+    // The same limit in every call: it belongs to the function, and another host thread may launch a larger row between a call's
+    // setting of its own and its launch.
+    if (const int rc = launch_code(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = bytes; cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)cluster; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, prm) == cudaSuccess ? FPKV_OK : FPKV_ELAUNCH;
+    return launch_code(cudaLaunchKernelEx(&cfg, kern, prm));
 }
 
 }  // namespace

@@ -544,9 +544,9 @@ int launch_prefix(const PoolView& pv, int layer, const void* q, long long q_stri
     }
     prm.rows_per_plane = pv.n_pages * pv.P;
     auto launch = [&](auto kern) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return FPKV_ELAUNCH;
+        if (const int rc = launch_code(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem))) return rc;
         kern<<<prefix_ctas(), kThreads, kSmem, stream>>>(q_map, kv_map, prm);
-        return cudaGetLastError() == cudaSuccess ? FPKV_OK : FPKV_ELAUNCH;
+        return launch_code(cudaGetLastError());
     };
     if (pv.dtype == FPKV_BF16) return pv.D == 128 ? launch(shared_prefix_kernel<__nv_bfloat16, 128>) : launch(shared_prefix_kernel<__nv_bfloat16, 64>);
     return pv.D == 128 ? launch(shared_prefix_kernel<__half, 128>) : launch(shared_prefix_kernel<__half, 64>);

@@ -1,11 +1,14 @@
 """GPU: token sampling against a 64-bit computation on the host."""
 
+import ctypes
 import math
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
+from fpkv import _lib
 from fpkv.sampling import sample
 
 pytestmark = pytest.mark.gpu
@@ -262,3 +265,51 @@ def test_uniform_numbers_out_of_range(V, dtype):
             want = sample(x, torch.zeros(4, device="cuda"), **kw)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (uv, kw)
             assert (got[0] >= 0).all() and (got[0] < V).all() and (got[0][1:] >= V - 20).all()
+
+
+THREADS_SOURCE = r"""
+#include <pthread.h>
+#include <stdint.h>
+typedef int (*sample_fn)(const void*, int32_t, int64_t, int32_t, int32_t, const float*, const float*, const int32_t*, const float*,
+                         const float*, int64_t*, float*, void*);
+struct job { sample_fn f; const void* x; int vocab; const float* u; int64_t* token; void* stream; int n, refused; };
+static void* run(void* p) {
+    struct job* j = p;
+    for (int i = 0; i < j->n; ++i)
+        j->refused += j->f(j->x, 0, j->vocab, 1, j->vocab, j->u, 0, 0, 0, 0, j->token, 0, j->stream) != 0;
+    return 0;
+}
+int sample_in_threads(sample_fn f, int threads, const void** x, const int* vocab, const float* u, int64_t** token, void** stream, int n) {
+    pthread_t t[8];
+    struct job j[8];
+    int refused = 0;
+    for (int i = 0; i < threads; ++i) {
+        struct job k = {f, x[i], vocab[i], u, token[i], stream[i], n, 0};
+        j[i] = k;
+        if (pthread_create(&t[i], 0, run, &j[i])) return -1;
+    }
+    for (int i = 0; i < threads; ++i) { pthread_join(t[i], 0); refused += j[i].refused; }
+    return refused;
+}
+"""
+
+
+def test_host_threads_with_rows_of_different_lengths(tmp_path):
+    """Launches of much and of little shared memory from threads without Python between the calls: none is refused."""
+    (tmp_path / "threads.c").write_text(THREADS_SOURCE)
+    subprocess.run(["gcc", "-O2", "-shared", "-fPIC", str(tmp_path / "threads.c"), "-o", str(tmp_path / "threads.so"), "-lpthread"], check=True)
+    call = ctypes.CDLL(str(tmp_path / "threads.so")).sample_in_threads
+    vocab, n, g = [64] * 6 + [300000] * 2, 5000, gen(2)
+    x = [logits_of(1, v, torch.float32, g) for v in vocab]
+    u = torch.full((1,), 0.5, device="cuda")
+    token = [torch.empty(1, dtype=torch.int64, device="cuda") for _ in vocab]
+    streams = [torch.cuda.Stream() for _ in vocab]
+    torch.cuda.synchronize()
+    pointers = lambda p: (ctypes.c_void_p * len(vocab))(*p)
+    refused = call(ctypes.cast(_lib.lib.fpkv_sample, ctypes.c_void_p), len(vocab), pointers([t.data_ptr() for t in x]),
+                   (ctypes.c_int * len(vocab))(*vocab), ctypes.c_void_p(u.data_ptr()), pointers([t.data_ptr() for t in token]),
+                   pointers([s.cuda_stream for s in streams]), n)
+    torch.cuda.synchronize()
+    assert refused == 0
+    for t, row in zip(token, x):
+        assert t.item() == reference(row, u)[0][0]
