@@ -265,19 +265,27 @@ class SlotState:
         """Draw every row's next token (``fpkv.sampling.sample``) and move the
         batch on (``advance``).  Device work only, in the order a captured decode
         step has it.  Returns (token, logprob) of the bucket's rows.  A row whose
-        logits allow nothing gets token -1: it is for the caller to end it."""
+        logits allow nothing gets token -1 and stays as it is, position and last
+        token, so that a step that runs before the caller ends it reads valid
+        inputs."""
         token, logprob = sample(logits, uniform, temperature, top_k, top_p, min_p)
-        self.advance(bucket, token)
+        self._advance(bucket, token, token[:bucket] >= 0)
         return token, logprob
 
     def advance(self, bucket: int, next_token: Tensor):
         """After sampling: every live row of the batch moves on by one token.  Device work only, no
         host value involved; padding rows (slot 0) stay at zero."""
+        self._advance(bucket, next_token.reshape(-1), None)
+
+    def _advance(self, bucket: int, next_token: Tensor, drawn: Tensor | None):
+        """``advance``, but for the rows where ``drawn`` is false."""
         bi = self.batch_idx[:bucket]
-        live = bi > 0
+        live, token = bi > 0, next_token[:bucket]
+        if drawn is not None:
+            live, token = live & drawn, torch.where(drawn, token, self.last_token[bi])
         self.input_pos.index_add_(0, bi, live.to(torch.int32))
         self.rope_pos_t.index_add_(0, bi, live.to(torch.int64))
-        self.last_token.index_copy_(0, bi, torch.where(live, next_token.reshape(-1)[:bucket], torch.zeros_like(bi)))
+        self.last_token.index_copy_(0, bi, torch.where(bi > 0, token, torch.zeros_like(bi)))
 
 
 # ------------------------------------------------------------- step planning

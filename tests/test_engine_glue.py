@@ -40,6 +40,20 @@ def test_slot_state_one_upload_per_step():
     assert m.batch_idx.tolist() == [3] and m.input_pos.tolist() == [42]
 
 
+def test_rows_that_allow_no_token_stay_where_they_are(monkeypatch):
+    st = SlotState(8, "cpu")
+    for slot in (3, 5, 6):
+        st.begin(slot, 10 * slot, 10 * slot + 1, 900 + slot)
+    st.stage([5, 3, 6], bucket=5)
+    drawn = torch.tensor([11, -1, 13, -1, 14]), torch.tensor([-0.5, -float("inf"), -0.25, -float("inf"), -1.0])
+    monkeypatch.setattr("fpkv.engine_glue.sample", lambda *a: drawn)
+    token, logprob = st.sample(5, torch.zeros(5, 32), torch.zeros(5))
+    assert token.tolist() == [11, -1, 13, -1, 14] and logprob is drawn[1]      # the caller sees which
+    bi, pos, rope, ids = st.step_inputs(5)
+    assert bi.tolist() == [5, 3, 6, 0, 0] and ids.tolist() == [11, 903, 13, 0, 0]
+    assert pos.tolist() == [51, 30, 61, 0, 0] and rope.tolist() == [52, 31, 62, 0, 0]
+
+
 def test_planner_mixes_prefill_chunks_with_decode_rows():
     c = PagedKVCache(40, 16, 6, 1, 64, 1, torch.float32, "cpu")             # 39 usable pages of 16 tokens
     pl = MixedStepPlanner(c, chunk_tokens=64, prefill_token_budget=96)
