@@ -383,7 +383,8 @@ sample_kernel(const SampleParams prm)
 
     // ---- bins go by the distance from the maximum in 32 bits, which does not decrease as the value falls ------------
     const float fmx = __uint_as_float(bits_of(kmax)), fslope = (float)slope;
-    auto distance = [&](uint32_t bits) { return key_of(bits) == kmax ? 0.f : fminf(fmx - __uint_as_float(bits), 3e38f); };
+    // Cut off where one over it is still a normal number, for the bins divide by it.
+    auto distance = [&](uint32_t bits) { return key_of(bits) == kmax ? 0.f : fminf(fmx - __uint_as_float(bits), 8e37f); };
     // Images around the value at a distance from the maximum, a few roundings to either side.
     auto near = [&](float d, bool above) {
         const float x_ = fmx - d, slack = 4e-7f * (fabsf(fmx) + d);
@@ -566,13 +567,8 @@ sample_kernel(const SampleParams prm)
         for (int o = 16; o > 0; o >>= 1) { const unsigned long long y = __shfl_xor_sync(0xffffffffu, got, o); got = y > got ? y : got; }
         return got;
     };
-    // The one image that the entries of fine bin b at or above thr share, or 0 if they differ.
-    auto only_value = [&](int b, unsigned long long thr) -> uint32_t {
-        uint32_t lo = 0xffffffffu, hi = 0;
-        each([&](uint32_t bits, int i) {
-            const uint32_t key = key_of(bits);
-            if (key >= k_first && key <= k_last && at_or_above(key, i, thr) && fine_of(key) == b) { lo = min(lo, key); hi = max(hi, key); }
-        });
+    // Smallest and largest image over the cluster.
+    auto extremes = [&](uint32_t& lo, uint32_t& hi) {
         lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) { sh.red_u[warp] = lo; sh.red_v[warp] = hi; }
         __syncthreads();
@@ -581,6 +577,18 @@ sample_kernel(const SampleParams prm)
         if (tid == 0) { sh.pub_low = lo; sh.pub_bound = hi; }
         cluster_sync();
         lo = __reduce_min_sync(0xffffffffu, peer(&sh.pub_low, from)); hi = __reduce_max_sync(0xffffffffu, peer(&sh.pub_bound, from));
+    };
+    // Narrows the fine bins down to the images that the entries of bin b at or above thr have, and returns the one they share, or
+    // 0 if they differ.  What is there is narrower than the bin by far where some entries lie far away -- masked by a large
+    // finite value, say -- and all others in one bin.
+    auto narrow = [&](int b, unsigned long long thr) -> uint32_t {
+        uint32_t lo = 0xffffffffu, hi = 0;
+        each([&](uint32_t bits, int i) {
+            const uint32_t key = key_of(bits);
+            if (key >= k_first && key <= k_last && at_or_above(key, i, thr) && fine_of(key) == b) { lo = min(lo, key); hi = max(hi, key); }
+        });
+        extremes(lo, hi);
+        span(lo, hi);
         return lo == hi ? lo : 0u;
     };
 
@@ -606,10 +614,24 @@ sample_kernel(const SampleParams prm)
         };
         bool all_kept = false, done = false;
         if (bounded && 4 * k <= 3 * kCand) {
-            // The k-th largest of the threads' largest values has k entries at or above it, and hardly more: collect those.
-            count([&] { if (top > kKeyNone) atomicAdd(&sh.hist[fine_of(top)], 1u); });
-            find(0);
-            const uint32_t from_key = edge(j);
+            // The k-th largest of the threads' largest values has k entries at or above it, and hardly more: collect those.  A bin
+            // of many values is narrowed down to them.
+            uint32_t from_key = 0, before = 0;
+            for (int turn = 0;; ++turn) {
+                const bool counted = top >= k_first && top <= k_last;
+                count([&] { if (counted) atomicAdd(&sh.hist[fine_of(top)], 1u); });
+                find(before);
+                if (j < 0) break;
+                from_key = edge(j);
+                if (in_j <= 64u || turn == 2) break;
+                const bool here = counted && fine_of(top) == j;
+                uint32_t lo = here ? top : 0xffffffffu, hi = here ? top : 0u;
+                extremes(lo, hi);
+                from_key = max(from_key, lo);
+                if (lo == hi) break;
+                before = until_j;
+                span(lo, hi);
+            }
             each([&](uint32_t bits, int i) { if (key_of(bits) >= from_key) collect(number(key_of(bits), i)); });
             done = gather() <= kCand && j >= 0;
             if (done) listed = (int)k;
@@ -617,6 +639,7 @@ sample_kernel(const SampleParams prm)
                 cluster_sync();                          // peers have read the number of entries
                 if (tid == 0) sh.n_list = 0;
                 __syncthreads();
+                span(from_key, kmax);                    // which holds k entries
             }
         }
         if (!done) {
@@ -626,11 +649,9 @@ sample_kernel(const SampleParams prm)
                 find(before);
                 if (j < 0) { all_kept = turn == 0; break; }              // fewer than k entries above -inf: no limit
                 if (in_j <= (uint32_t)kCand) break;
-                one = only_value(j, everything);
-                if (one != 0 || turn == 3) break;
-                // too many in one bin, of different values: the bin becomes the range
+                one = narrow(j, everything);
                 before = until_j;
-                span(edge(j), edge(j - 1) - 1u);
+                if (one != 0 || turn == 3) break;
             }
             if (j >= 0 && in_j <= (uint32_t)kCand) {
                 const uint32_t from_key = edge(j), to_key = edge(j - 1);
@@ -785,11 +806,10 @@ sample_kernel(const SampleParams prm)
                 if (sh.at[12] && sh.at[10] >= 0 && in_j + sh.at[11] <= kCand) p_hi = sh.at[10];
                 break;
             }
-            tie = only_value(j, threshold);
+            tie = narrow(j, threshold);
             lost = tie == 0 && turn == 3;
             if (tie != 0 || lost) break;
             mass_before = __int_as_float(sh.at[5]);
-            span(edge(j), edge(j - 1) - 1u);
         }
     }
 
