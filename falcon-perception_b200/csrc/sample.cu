@@ -138,7 +138,7 @@ struct __align__(16) Shared {
     unsigned long long red_l[kWarps];
     unsigned long long pub_max;
     float wide_sum[kWide];                               // published: the CTA's sums over the wide bins
-    uint32_t pub_low, pub_bound, pub_n, pub_ties;
+    uint32_t pub_low, pub_bound, pub_tops, pub_n, pub_ties;
     uint32_t red_u[kWarps], red_v[kWarps];
     uint32_t n_list;
     int at[16];
@@ -265,7 +265,8 @@ sample_kernel(const SampleParams prm)
     // one number a entry that orders the row
     auto number = [&](uint32_t key, int i) { return ((unsigned long long)key << 32) | (uint32_t)~i; };
 
-    // ---- 1. the slice; its largest entry, its smallest finite value, the smallest of its threads' largest values ----
+    // ---- 1. the slice; its largest entry, its smallest value above -inf, the smallest of its threads' largest values, and how
+    // many threads have one (the last slice is short, and masked ones read nothing else than -inf) ----
     const float temp = prm.temperature != nullptr ? prm.temperature[row] : 1.f;
     const float p_top = prm.top_p != nullptr ? prm.top_p[row] : 1.f;
     const int k_top = prm.top_k != nullptr ? prm.top_k[row] : 0;
@@ -288,7 +289,7 @@ sample_kernel(const SampleParams prm)
             }
         }
         if (top > kKeyNone) best = number(top, at);
-        bound = top;                                     // 0 or the image of -inf where the thread has nothing
+        if (top > kKeyNone) bound = top;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -297,7 +298,8 @@ sample_kernel(const SampleParams prm)
     }
     low = __reduce_min_sync(0xffffffffu, low);
     bound = __reduce_min_sync(0xffffffffu, bound);
-    if (lane == 0) { sh.red_l[warp] = best; sh.red_u[warp] = low; sh.red_v[warp] = bound; }
+    uint32_t tops = __popc(__ballot_sync(0xffffffffu, top > kKeyNone));
+    if (lane == 0) { sh.red_l[warp] = best; sh.red_u[warp] = low; sh.red_v[warp] = bound; sh.at[warp] = (int)tops; }
     if (tid < 16) sh.exp_table[tid] = exp2((double)tid * 0.0625);
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
@@ -312,7 +314,8 @@ sample_kernel(const SampleParams prm)
         }
         low = __reduce_min_sync(0xffffffffu, low);
         bound = __reduce_min_sync(0xffffffffu, bound);
-        if (lane == 0) { sh.pub_max = best; sh.pub_low = low; sh.pub_bound = bound; }
+        tops = __reduce_add_sync(0xffffffffu, lane < kWarps ? (uint32_t)sh.at[lane] : 0u);
+        if (lane == 0) { sh.pub_max = best; sh.pub_low = low; sh.pub_bound = bound; sh.pub_tops = tops; }
     }
     cluster_sync();
     best = peer(&sh.pub_max, from);
@@ -323,6 +326,7 @@ sample_kernel(const SampleParams prm)
     }
     low = __reduce_min_sync(0xffffffffu, peer(&sh.pub_low, from));
     bound = __reduce_min_sync(0xffffffffu, peer(&sh.pub_bound, from));
+    tops = __reduce_add_sync(0xffffffffu, lane < (int)C ? peer(&sh.pub_tops, from) : 0u);
     best = __shfl_sync(0xffffffffu, best, 0);
     const uint32_t kmax = (uint32_t)(best >> 32);
     if (best == 0 || !(temp > 0.f)) {                    // the same for the whole cluster
@@ -597,8 +601,8 @@ sample_kernel(const SampleParams prm)
     // ---- 2. top-k ------------------------------------------------------------------
     if (by_k) {
         const uint32_t k = (uint32_t)k_top;
-        // Every thread of the cluster that read anything has an entry at or above `bound`.
-        const bool bounded = k <= kThreads * C && bound > kKeyNone;
+        // Every one of the `tops` threads has an entry at or above `bound`.
+        const bool bounded = k <= tops;
         span(bounded ? bound : low, kmax);
         int j = -1; uint32_t in_j = 0, until_j = 0;
         // The bin of the k-th of what was counted, behind `before` others.

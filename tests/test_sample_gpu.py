@@ -374,3 +374,22 @@ def test_masks_by_finite_values_take_the_ordinary_path():
         for v in (torch.finfo(x.dtype).min, -1e30):
             t = microseconds(x.masked_fill(gone, v), u, kt)
             assert t < 2.5 * t_inf, f"k {k}, masked by {v}: {t:.1f} us against {t_inf:.1f}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bfloat16", "float32"])
+def test_small_k_where_threads_have_nothing(dtype):
+    """Short last slices and rows of mostly -inf: k below, at and above the number of threads that have an entry at all."""
+    g = gen(12)
+    for B, V in ((1, 32000), (40, 32000), (2, 4100), (3, 700)):
+        x = logits_of(B, V, dtype, g)
+        u, r = torch.rand(B, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda")
+        for left in (1, 9, 50, 51, 200):
+            y = torch.full_like(x, -math.inf)
+            at = torch.randperm(V, generator=g, device="cuda")[:left]
+            y[:, at] = x[:, at]
+            y[0, :left] = x[0, :left]; y[0, left:] = -math.inf          # all of them with a few threads
+            for k in (1, 8, 50, 51, 384):
+                kt = torch.full((B,), k, dtype=torch.int32, device="cuda")
+                check(y, u, k=kt, what=f"{left} left, k {k}"); check(y, u, k=kt, p=r, what=f"{left} left, k {k}, p")
+        for k in (50, 384, 385, 600):
+            check(x, u, k=torch.full((B,), k, dtype=torch.int32, device="cuda"), what=f"k {k}")
