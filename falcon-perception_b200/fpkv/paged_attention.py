@@ -616,11 +616,14 @@ class PagedKVCache(KVCacheBase):
         one prefix next to each other); ``rows``: the padded batch size, rows
         beyond ``slots`` are in no group.  Host work and one small copy: make it
         when the batch changes, pass it to every layer of every step until then.
-        ``into`` refills an earlier record in place (same number of rows, no more
-        groups than it has room for), so that a captured graph sees the new batch."""
+        ``into`` refills an earlier record in place (same number of rows), so that a
+        captured graph sees the new batch.  Of more groups than the record has room
+        for (a new one: 1024), those are kept that save the most pages; the other
+        rows are in no group."""
         slots = [int(s) for s in slots]
         rows = len(slots) if rows is None else int(rows)
         assert rows >= len(slots), "the padded batch is smaller than the batch"
+        assert into is None or into.row_group.shape[0] == rows, "the record is one of another number of rows"
         found, row_group, i = [], [-1] * rows, 0
         while i < len(slots):
             first = self.page_table_cpu[slots[i]]
@@ -635,13 +638,15 @@ class PagedKVCache(KVCacheBase):
                     break
                 n, j = m, j + 1
             if j - i > 1:
-                row_group[i:j] = [len(found)] * (j - i)
                 found.append((i, j - i, n, 0))
             i = j
+        room = _lib.MAX_GROUPS if into is None else into.n_groups
+        if len(found) > room:                       # the first of those that save equally much, in the order of the rows
+            found = sorted(sorted(found, key=lambda g: -(g[1] - 1) * g[2])[:room])
+        for k, (i, n, _, _) in enumerate(found):
+            row_group[i:i + n] = [k] * n
         if into is not None:
-            assert into.row_group.shape[0] == rows and len(found) <= into.n_groups, "the record has no room for this batch"
-            found += [(0, 0, 0, 0)] * (into.n_groups - len(found))
-        assert len(found) <= _lib.MAX_GROUPS, f"more than {_lib.MAX_GROUPS} groups"
+            found += [(0, 0, 0, 0)] * (room - len(found))
         flat = torch.tensor([x for g in found for x in g] + row_group, dtype=torch.int32)
         if into is not None:
             n = 4 * into.n_groups

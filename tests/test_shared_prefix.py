@@ -207,3 +207,25 @@ def test_python_refusals():
             bad()
     with pytest.raises(RuntimeError, match="CUDA"):
         c.step_tables(i64, i32, i32, 8)
+
+
+def test_prefix_groups_beyond_the_room_left_out():
+    """A record has room for so many groups; those that save least are in none, in a new record and in a refilled one."""
+    n = _lib.MAX_GROUPS + 6
+    c = PagedKVCache(4 * n, 16, 3 * n, 1, 64, 1, torch.float32, "cpu")
+    slots, first = [], []
+    for i in range(n):
+        pages = 2 if i % 200 else 1                     # the groups of one page save least: 0, 200, ... 1000
+        a = c.allocate(); c.reserve(a, None, pages * 16)
+        first.append(len(slots)); slots += [a, c.share_prefix(a, pages * 16)]
+    g = c.prefix_groups(slots)
+    assert g.n_groups == _lib.MAX_GROUPS
+    kept = [i for i in range(n) if i % 200]
+    assert g.groups.tolist() == [[first[i], 2, 2, 0] for i in kept]
+    assert g.row_group.tolist() == [k for i in range(n) for k in 2 * [kept.index(i) if i % 200 else -1]]
+    small = c.prefix_groups(slots[:4], rows=8)           # room for two
+    assert small.n_groups == 2
+    c.prefix_groups(slots[:8], into=small)
+    assert small.groups.tolist() == [[2, 2, 2, 0], [4, 2, 2, 0]] and small.row_group.tolist() == [-1, -1, 0, 0, 1, 1, -1, -1]
+    with pytest.raises(AssertionError):
+        c.prefix_groups(slots[:2], into=small)           # another number of rows
