@@ -623,6 +623,7 @@ class PagedKVCache(KVCacheBase):
         slots = [int(s) for s in slots]
         rows = len(slots) if rows is None else int(rows)
         assert rows >= len(slots), "the padded batch is smaller than the batch"
+        assert all(0 <= s < self.max_batch_size for s in slots), "slot out of range"
         assert into is None or into.row_group.shape[0] == rows, "the record is one of another number of rows"
         found, row_group, i = [], [-1] * rows, 0
         while i < len(slots):

@@ -229,3 +229,12 @@ def test_prefix_groups_beyond_the_room_left_out():
     assert small.groups.tolist() == [[2, 2, 2, 0], [4, 2, 2, 0]] and small.row_group.tolist() == [-1, -1, 0, 0, 1, 1, -1, -1]
     with pytest.raises(AssertionError):
         c.prefix_groups(slots[:2], into=small)           # another number of rows
+
+
+def test_prefix_groups_refuse_slots_that_are_none():
+    c = cpu_cache()
+    a = c.allocate(); c.reserve(a, None, 40)
+    for bad in ([a, -1], [-1, -1], [a, c.max_batch_size]):
+        with pytest.raises(AssertionError):
+            c.prefix_groups(bad)
+    assert groups_of(c, [a, 0, 0]) == ([], [-1, -1, -1])         # padding is fine
