@@ -22,6 +22,8 @@ def _per_row(value, name: str, rows: int, dtype: torch.dtype, like: Tensor) -> T
     if value is None:
         return None
     if not isinstance(value, Tensor):
+        if dtype == torch.int32:                    # beyond the vocabulary: no limit, as for a tensor of int64
+            value = min(max(int(value), 0), like.shape[1])
         return torch.full((rows,), value, dtype=dtype, device=like.device)
     assert value.shape == (rows,), f"{name} must have one entry a row"
     assert value.device == like.device, f"{name} must be on the logits' device"

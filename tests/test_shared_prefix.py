@@ -11,7 +11,7 @@ from fpkv import _lib
 from fpkv.attention import CausalDecodeMask, PrefixGroups
 from fpkv.engine_glue import decoding_block_mask
 from fpkv.paged_attention import PagedKVCache
-from fpkv.sampling import sample
+from fpkv.sampling import _per_row, sample
 
 
 def cpu_cache(n_pages=64, page_size=16, slots=12):
@@ -238,3 +238,11 @@ def test_prefix_groups_refuse_slots_that_are_none():
         with pytest.raises(AssertionError):
             c.prefix_groups(bad)
     assert groups_of(c, [a, 0, 0]) == ([], [-1, -1, -1])         # padding is fine
+
+
+def test_top_k_as_a_number_of_any_size():
+    like = torch.zeros(3, 1000)
+    for k, want in ((2 ** 40, 1000), (2 ** 31, 1000), (1000, 1000), (7, 7), (0, 0), (-1, 0), (-2 ** 40, 0)):
+        got = _per_row(k, "top_k", 3, torch.int32, like)
+        assert got.dtype == torch.int32 and got.tolist() == [want] * 3
+        assert torch.equal(got, _per_row(torch.full((3,), k), "top_k", 3, torch.int32, like))
