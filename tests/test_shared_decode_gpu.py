@@ -374,3 +374,21 @@ def test_groups_with_common_rows_stay_inside_the_workspace(n):
     with pytest.raises(RuntimeError, match="bad slot"):
         c.check_status()
     check(out, lse, reference(c, 0, q, slots, last, 0.125))          # their group is the first one, which fits
+
+
+def test_records_of_another_form_are_refused():
+    c, slots, last, q = build(4, 2, 64, torch.bfloat16, [(2, [300, 301, 302])], ())
+    bi, ip = torch.tensor(slots, device="cuda"), torch.tensor(last, dtype=torch.int32, device="cuda")
+    for groups, row_group in ((torch.zeros(1, 3), torch.zeros(3)), (torch.zeros(4), torch.zeros(3)), (torch.zeros(2, 5)[:, :4], torch.zeros(3)),
+                              (torch.zeros(1, 4), torch.zeros(4)), (torch.zeros(1, 4), torch.zeros(6)[::2])):
+        g = c.prefix_groups(slots)
+        g.groups, g.row_group = (t.to(torch.int32).cuda() if t.is_contiguous() else torch.empty_strided(t.shape, t.stride(), dtype=torch.int32, device="cuda")
+                                 for t in (groups, row_group))
+        with pytest.raises(AssertionError):
+            c.decode_attention(0, q, bi, ip, shared=g)
+    g = c.prefix_groups(slots)
+    for name, t in (("groups", g.groups.cpu()), ("row_group", g.row_group.cpu()), ("groups", g.groups.long()), ("row_group", g.row_group.long())):
+        h = c.prefix_groups(slots)
+        setattr(h, name, t)
+        with pytest.raises(AssertionError):
+            c.decode_attention(0, q, bi, ip, shared=h)
