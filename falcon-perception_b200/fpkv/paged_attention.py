@@ -672,10 +672,11 @@ class PagedKVCache(KVCacheBase):
             q = q.contiguous()
             stride_b, stride_h = q.stride()[:2]
         groups, row_group = shared.groups, shared.row_group
-        assert groups.ndim == 2 and groups.shape[1] == 4, "prefix groups must be (n, 4)"
-        assert groups.device == row_group.device == q.device, "prefix groups must be on the cache's device"
-        assert groups.is_cuda and groups.is_contiguous() and groups.dtype is torch.int32, "prefix groups must be int32 on the device"
-        assert row_group.is_cuda and row_group.is_contiguous() and row_group.dtype is torch.int32, "prefix groups must be int32 on the device"
+        where = q.get_device()
+        assert groups.get_device() == where == row_group.get_device(), "prefix groups must be on the cache's device"
+        assert groups.dim() == 2 and groups.size(1) == 4, "prefix groups must be (n, 4)"
+        assert groups.dtype is torch.int32 is row_group.dtype and groups.is_contiguous() and row_group.is_contiguous(), \
+            "prefix groups must be contiguous and int32"
         key = (B, Hq, n_groups)
         size = self._shared_bytes.get(key)
         if size is None:
