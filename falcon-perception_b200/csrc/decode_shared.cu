@@ -11,6 +11,7 @@
 //    the other, in equal shares, one per WARP: a warp needs no other, so there is no barrier, and all have the same to do
 //    however the lengths differ.  A block is
 //        S^T = K Q^T   (16 keys x 8 heads),   O^T += V^T P^T   (dims x 8 heads)      in mma.sync.m16n8k16,
+//    with P rounded to the 16-bit type of V, as there, and the sums of P in 32 bits before that.
 //    K and V come by tensor copies (16 rows, 128-byte swizzle) into a ring of the warp's own, requested several blocks ahead
 //    and across rows: with only what fits the registers in flight, 12 warps an SM reached 3.7 TB/s.  The order of the
 //    contraction index and of the output's dims is free, so it is chosen such that every lane's 16-byte piece of a row is its

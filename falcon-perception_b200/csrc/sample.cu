@@ -23,9 +23,10 @@
 // 64-bit pipe has half the lanes of the 32-bit one, so the exponential is the table-and-polynomial one below: 12 operations.
 // No result depends on the order in which atomics arrive: counts are integers, collected entries are sorted.
 //
-// What bounds it: a few rows (1 x 65536 with top-p: 34 us) the chain of about ten barriers and lookups; many rows (512 x
-// 131072 in 32 bits, 268 MB, 41 us of memory) the instructions an entry takes: about 15 to load and compare it, 25 for the
-// wide bins, 10 for the counts, 50 for the 64-bit weight.
+// What bounds it: a few rows (1 x 65536 with top-p: 31 us) the chain of about ten barriers and lookups; many rows (512 x
+// 131072 in 32 bits, 268 MB, 41 us of memory, 537 us) the instructions an entry takes, 139 with these settings -- about 15 to
+// load and compare it, 25 for the wide bins, 10 for the counts, 50 for the 64-bit weight, and the searches -- which fill 52 % of
+// the issue slots of 29 warps an SM; the rest is waiting at barriers (a fifth of the stalls) and for the slice.
 
 #include "common.cuh"
 

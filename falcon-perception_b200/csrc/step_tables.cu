@@ -4,8 +4,9 @@
 // entries at most; the repeated scan costs less than a second launch would), then the CTAs share out
 // the packed tokens and the block-table entries.  A warp finds its first token's request by bisection in
 // shared memory, its other tokens go on from there, and a token's page takes one table read.  Bound by
-// the stores (32 bytes a packed token) on long rows and by the launch plus three dependent memory reads
-// (lengths, slot, page) on short ones.
+// instructions and the dependent reads of a token (slot, start, page) on long rows -- 512 requests, 790 K tokens:
+// 18.5 us, issue slots 53 % busy, while the 25 MB stored stay in L2 and would take 4 us -- and by the launch plus
+// three dependent memory reads (lengths, slot, page) on short ones.
 
 #include "common.cuh"
 

@@ -549,7 +549,8 @@ class PagedKVCache(KVCacheBase):
         followed by the attention call, ``falcon_perception/model.py:150-162``).
         Same results as the two separate calls; because the attention kernel
         knows that the append is what runs right before it, its set-up overlaps
-        the append instead of waiting for it.  With ``sinks`` (n_q_heads,) the
+        the append instead of waiting for it (not with ``shared``, whose kernels
+        start behind the append).  With ``sinks`` (n_q_heads,) the
         returned out is already ``out * sigmoid(lse - sinks)``, the gate of
         ``_post_attention`` (``model.py:122-128``); viewed as (B, 1, Hq*D) it is
         what the output projection takes.  ``shared`` as for ``decode_attention``."""
@@ -565,7 +566,12 @@ class PagedKVCache(KVCacheBase):
         batch_idx[b].  q (B,Hq,1,D) -> out (B,Hq,1,D) in q's dtype, lse (B,Hq,1)
         fp32.  Call after ``insert_kv`` of the same step, as the model does.
         ``shared`` (``prefix_groups`` of the batch's slots): leading pages that
-        rows have in common are read once for all of them; the result is the same.
+        rows have in common are read once for all of them.  The result is the same
+        but for the order of sums in 32 bits, as long as a prefix's values are
+        finite: where a position lies inside the prefix, an infinity or NaN behind it
+        that another row of the group sees makes NaN here too.  It pays with enough
+        rows or keys a group (64 rows over 8192 keys 59 us instead of 209); small
+        ones lose to the call without it (4 rows over 512 keys 25 us against 16).
         Pools that ``fpkv_decode_attn_shared`` does not take (fp32, split layout,
         page sizes other than 128, more than 16 query heads per stored head) are
         served row by row as without it, as are pools of 2^31 or more rows over all

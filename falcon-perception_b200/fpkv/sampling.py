@@ -41,9 +41,9 @@ def sample(logits: Tensor, uniform: Tensor, temperature: Tensor | float | None =
     """One token a row.  ``logits`` (B, V) in fp32, bf16 or fp16 on a CUDA device
     (rows may be strided); ``uniform`` (B,) float32 in [0, 1) (below it or NaN
     counts as 0, beyond it draws the last kept entry).  The settings are
-    one number for all rows or one a row: ``temperature`` (<= 0: greedy, the
-    lowest index among equal logits), ``top_k`` (<= 0: no limit), ``top_p`` (>= 1:
-    no limit), ``min_p`` (<= 0: no limit).
+    one number for all rows or one a row: ``temperature`` (<= 0 or subnormal:
+    greedy, the lowest index among equal logits), ``top_k`` (<= 0: no limit),
+    ``top_p`` (>= 1: no limit), ``min_p`` (<= 0 or subnormal: no limit).
 
     Entries are ordered by logit, ties by lowest index.  top_k keeps the first k;
     top_p of those the shortest leading run whose probability reaches top_p (at

@@ -398,8 +398,9 @@ FPKV_API int fpkv_decode_attn_static(const fpkv_pool* pool, int32_t layer,
  * requests about one picture or document, their first pages mapped to the same
  * physical pages (allocator record "share").  It has no counterpart in the
  * reference.  Same results and conventions as fpkv_decode_attn on the same
- * arguments; the keys of a shared prefix are read once for all rows of its
- * group instead of once a row.
+ * arguments, but for the order of sums in 32 bits and the values below; the keys
+ * of a shared prefix are read once for all rows of its group instead of once a
+ * row.
  *   groups     device int32 [n_groups][4], 16-byte aligned, each {first row, rows,
  *              shared pages, 0}: batch rows first .. first+rows-1 all map logical
  *              pages 0 .. shared-1 to the same physical pages (the kernel reads
@@ -494,10 +495,12 @@ FPKV_API int fpkv_step_tables(const fpkv_pool* pool, const int64_t* slots, const
  *                vocab contiguous; aligned to its element size
  *   uniform      device float [rows], in [0, 1).  < 0 or NaN counts as 0, >= 1
  *                draws the last kept entry with any weight
- *   temperature  device float [rows] or NULL (1).  <= 0 or NaN: greedy, logprob 0
+ *   temperature  device float [rows] or NULL (1).  <= 0, subnormal or NaN: greedy,
+ *                logprob 0
  *   top_k        device int32 [rows] or NULL.  <= 0: no limit
  *   top_p        device float [rows] or NULL.  >= 1 or NaN: no limit; <= 0: one entry
- *   min_p        device float [rows] or NULL.  <= 0 or NaN: no limit; > 1 counts as 1
+ *   min_p        device float [rows] or NULL.  <= 0, subnormal or NaN: no limit; > 1
+ *                counts as 1
  *   token        device int64 [rows];  logprob  device float [rows] or NULL
  * A NaN logit counts as -inf; entries of -inf are never drawn; a row with
  * nothing else gives token -1, logprob -inf.  Entries of +inf share the mass.

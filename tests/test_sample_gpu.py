@@ -393,3 +393,15 @@ def test_small_k_where_threads_have_nothing(dtype):
                 check(y, u, k=kt, what=f"{left} left, k {k}"); check(y, u, k=kt, p=r, what=f"{left} left, k {k}, p")
         for k in (50, 384, 385, 600):
             check(x, u, k=torch.full((B,), k, dtype=torch.int32, device="cuda"), what=f"k {k}")
+
+
+def test_subnormal_settings_count_as_zero():
+    g = gen(31)
+    x = logits_of(6, 5000, torch.float32, g)
+    x[0, 100] = x[0, 200] = 99.0                         # greedy: the first of them
+    u = torch.rand(6, generator=g, device="cuda")
+    full = lambda v: torch.full((6,), v, device="cuda")
+    got, want = sample(x, u, temperature=full(1e-40)), sample(x, u, temperature=full(0.0))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[0][0] == 100
+    got, want = sample(x, u, min_p=full(1e-40)), sample(x, u)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
