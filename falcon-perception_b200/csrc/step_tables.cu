@@ -65,13 +65,15 @@ step_tables_kernel(const StepParams prm)
             if (w < warp) { pa += w_al[w]; pn += w_ln[w]; }
             base_al += w_al[w]; base_ln += w_ln[w];
         }
-        if (r < N) { first[r] = sat(pa + xa - al); cum[r] = sat(pn + xn - n); }
+        if (r < N) {
+            first[r] = sat(pa + xa - al); cum[r] = sat(pn + xn - n);
+            // tokens past the row's end; a run's gap, or padding, may reach beyond it
+            if (blockIdx.x == 0 && n > 0 && pa + xa - al + n > prm.row_tokens && prm.slots[r] != 0) raise_status(prm.status, FPKV_STATUS_BAD_POS);
+        }
         __syncthreads();
     }
     if (tid == 0) { first[N] = sat(base_al); cum[N] = sat(base_ln); }
     __syncthreads();
-    const bool too_long = base_al > prm.row_tokens;
-    if (too_long && blockIdx.x == 0 && tid == 0) raise_status(prm.status, FPKV_STATUS_BAD_POS);
 
     const int step = gridDim.x * kStepThreads, at = blockIdx.x * kStepThreads + tid;
     // ---- the packed row ------------------------------------------------------

@@ -225,3 +225,20 @@ def test_a_serving_step_together():
             if step < 5:
                 assert (ha[step][i] - hb[step][i]).abs().max() <= 2.0 ** -6 * hb[step][i].abs().max()
     assert sum(a == b for a, b in zip(sum(ta, []), sum(tb, []))) >= 24
+
+
+def test_rows_that_end_behind_the_last_token():
+    """The last request's run need not fit, only its tokens; nor need a padding request, whose tokens are pads."""
+    c, slots = cache_for([300, 300])
+    for align in (16, 128):
+        check(c, slots, [0, 7], [100, 33], -(-100 // align) * align + 33, align=align)
+        check(c, slots[:1], [0], [5], 5, align=align)
+        check(c, slots + [0], [0, 7, 0], [100, 33, 50], -(-100 // align) * align + 40, align=align)
+        check(c, slots, [0, 7], [100, 0], 100, align=align)
+    c.check_status()
+    check(c, slots, [0, 7], [100, 33], 128 + 32)
+    with pytest.raises(RuntimeError, match="bad position"):
+        c.check_status()
+    check(c, slots, [0, 7], [100, 33], 99)
+    with pytest.raises(RuntimeError, match="bad position"):
+        c.check_status()
