@@ -241,6 +241,10 @@ class PagedKVCache(KVCacheBase):
         n = len(self._pending)
         if n == 0:
             return
+        index = self._dev.index if self._dev.index is not None else self._page_table.device.index
+        if torch.cuda.current_device() != index:    # a launch goes to the current device, whatever its pointers are of
+            with torch.cuda.device(index):
+                return self._flush_tables()
         if n > self._ops_cap:                       # a step with more calls than ever before: grow (allocates)
             torch.cuda.current_stream(self._dev).synchronize()
             self._ops_cap = max(n, 2 * self._ops_cap)
@@ -554,6 +558,9 @@ class PagedKVCache(KVCacheBase):
         returned out is already ``out * sigmoid(lse - sinks)``, the gate of
         ``_post_attention`` (``model.py:122-128``); viewed as (B, 1, Hq*D) it is
         what the output projection takes.  ``shared`` as for ``decode_attention``."""
+        if shared is not None and q.is_cuda and torch.cuda.current_device() != q.get_device():
+            with torch.cuda.device(q.get_device()):
+                return self.decode_step(layer_id, q, k, v, batch_idx, input_pos, sm_scale, out, lse, sinks, shared)
         B = q.shape[0]
         self.assign(layer_id, batch_idx, input_pos.reshape(B, 1), k, v)
         return self.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks=sinks, shared=shared,
@@ -576,6 +583,9 @@ class PagedKVCache(KVCacheBase):
         page sizes other than 128, more than 16 query heads per stored head) are
         served row by row as without it, as are pools of 2^31 or more rows over all
         heads and a scale that is not positive."""
+        if shared is not None and q.is_cuda and torch.cuda.current_device() != q.get_device():
+            with torch.cuda.device(q.get_device()):
+                return self.decode_attention(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, _after_append)
         B, Hq, S, D = q.shape
         assert S == 1, "decode attention takes one query token per row"
         assert D == self.head_dim and Hq % self.n_heads == 0, "head layout must match the pool"
@@ -660,7 +670,7 @@ class PagedKVCache(KVCacheBase):
             into.groups.copy_(flat[:n].view(-1, 4))
             into.row_group.copy_(flat[n:])
             return into
-        flat = flat.to(self._dev)
+        flat = flat.to(self._page_table.device)
         return PrefixGroups(flat[:4 * len(found)].view(-1, 4), flat[4 * len(found):])
 
     def _shared_supported(self, B: int, Hq: int) -> bool:
@@ -670,9 +680,6 @@ class PagedKVCache(KVCacheBase):
                 and 2 * self.n_heads * self.n_pages * self.page_size < 1 << 31)
 
     def _decode_shared(self, layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups):
-        if torch.cuda.current_device() != q.device.index:
-            with torch.cuda.device(q.device):
-                return self._decode_shared(layer_id, q, batch_idx, input_pos, sm_scale, out, lse, sinks, shared, B, Hq, n_groups)
         stride_b, stride_h = q.stride()[:2]
         if stride_b == 0 or stride_h == 0:          # the kernel's tensor map has no room for a repeated row
             q = q.contiguous()

@@ -246,3 +246,65 @@ def test_top_k_as_a_number_of_any_size():
         got = _per_row(k, "top_k", 3, torch.int32, like)
         assert got.dtype == torch.int32 and got.tolist() == [want] * 3
         assert torch.equal(got, _per_row(torch.full((3,), k), "top_k", 3, torch.int32, like))
+
+
+def test_launches_go_to_the_caches_device(monkeypatch):
+    """With another device current, queued table edits and calls with groups, those that are served row by row among them, switch
+    to the cache's (stand-ins for CUDA: the device current at the launch is what counts)."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, d):
+            self.d = d if isinstance(d, int) else d.index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.d
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    class Event:
+        def record(self, stream):
+            pass
+
+        def synchronize(self):
+            pass
+
+    class Stop(Exception):
+        pass
+
+    class Query:
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+
+        @property
+        def shape(self):
+            seen.append(current[0])
+            raise Stop
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: None)
+    monkeypatch.setattr("fpkv.paged_attention._stream", lambda d: 0)
+
+    class Library:
+        @staticmethod
+        def fpkv_alloc_step(*a):
+            seen.append(current[0])
+            return 0
+
+    c = cpu_cache()
+    c._dev = torch.device("cuda", 1)
+    c._ops_cap, c._ops_turn, c._alloc = 8, 0, _lib.FpkvAllocState()
+    c._ops_host, c._ops_done, c._ops_dev = [torch.empty(8, 4, dtype=torch.int32)] * 2, [Event(), Event()], torch.empty(8, 4, dtype=torch.int32)
+    a = c.allocate(); c.reserve(a, None, 40); c.share_prefix(a, 32)
+    monkeypatch.setattr(_lib, "lib", Library)
+    c.flush_tables()
+    assert seen == [1] and current == [0] and not c._pending
+    g = PrefixGroups(torch.zeros((0, 4), dtype=torch.int32), torch.full((1,), -1, dtype=torch.int32))
+    for call in (lambda: c.decode_attention(0, Query(), None, None, shared=g), lambda: c.decode_step(0, Query(), None, None, None, None, shared=g)):
+        with pytest.raises(Stop):
+            call()
+    assert seen == [1, 1, 1] and current == [0]
