@@ -15,9 +15,10 @@
 // through in two halves of 64 keys with separate score columns,
 //     S = Q K^T   128x64xD,   A = Q (shared), B = 64 rows of the K tile (shared)
 //     O += P V    128xDx64,   A = P (tensor memory, over the first half of the S columns), B = 64 rows of the V tile
-// with P rounded to 16 bits, the type the MMA takes it in (at most half a step each, as the decode and prefill kernels round it;
-// the row sums are those of P before the rounding, in 32 bits), so that four chains S -> softmax -> P V -> next S are in flight.  Warp 8 issues the copies, warps 9 and 10 the MMAs, warp 11
-// prepares the next piece and, 64 key tiles ahead, the pool rows of its pages.
+// with P rounded to 16 bits, the type the MMA takes it in (at most half a step each, as the decode and prefill kernels
+// round it; the row sums are those of P before the rounding, in 32 bits), so that four chains
+// S -> softmax -> P V -> next S are in flight.  Warp 8 issues the copies, warps 9 and 10 the MMAs, warp 11 prepares the
+// next piece and, 64 key tiles ahead, the pool rows of its pages.
 //
 // Bound: with at most 128 query rows a segment by the bytes of K and V (a tile's MMAs take 1040 clocks, its exponentials
 // 1024, its 64 KiB at the SM's share of memory 2800); with more by the MMAs and exponentials.
